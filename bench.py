@@ -826,7 +826,7 @@ def torch_mode_leg(torch, np, gcodec, codec, x, n, bits, words, lanes, dev, pgen
         "mt19937_parallel_ms": ms_gen, "mt19937_parallel_draws_per_s": n / (ms_gen * 1e-3),
         "mt19937_serial_draws_per_s": 10_000_000 / (ms_ser * 1e-3),
         "note": "torch-CPU-generator (MT19937) draws, bit-exact with compressors.py: jump-ahead parallel "
-                "generators on two high-priority side streams (phase 1 = sequence + jumps + a jump straight to "
+                "generators on two side streams (phase 1 = sequence + jumps + a jump straight to "
                 "the end state, phase 2 = the generators) -> encode from the draws on the caller's stream; "
                 "torch's state is written back every call (host sync) as soon as phase 1 is done; back to back, "
                 "the next same-size call's run is enqueued behind this one and used only if torch's generator "

@@ -986,8 +986,6 @@ MT_MULTI_CALLS = 8
 # jump work, which shares the chip with the encodes (DESIGN_HISTORY section 7)
 MT_PIPE_GENERATORS = None
 MT_WAIT_NEXT_JUMPS = False  # consumers also wait for the speculative run's jumps (mt19937_draws)
-# side-stream priorities ("high" or "normal") of the jumps and of the generators
-MT_SIDE_PRIORITY = ("high", "high")
 
 
 def mt_pipe_generators(count: int, multi: bool = False) -> int:
@@ -1010,17 +1008,18 @@ def mt_pipe_generator_draws(count: int, multi: bool = False) -> int:
 
 
 def _mt_side(device):
-    """High-priority streams: one for the jumps (LDS-bound; they also produce
-    the end state, so run c+1's jumps follow run c's) and one per slot for the
+    """Side streams: one for the jumps (LDS-bound; they also produce the end
+    state, so run c+1's jumps follow run c's) and one per slot for the
     generators (latency-bound), so the generators of the runs in flight run
     side by side instead of one after another.  The encodes the draws feed
-    fill the CUs they leave idle."""
+    fill the CUs they leave idle.  All at the default priority: queues of
+    different priorities have stalled for good on this hardware, and the
+    measured time of a call does not depend on them (0.319-0.327 ms for all
+    four combinations, profiles/r06w_torch_priority.log)."""
     s = _MT_SIDE.get(device.index)
     if s is None:
-        lo, hi = torch.cuda.Stream.priority_range()
-        pj, pg = (min(lo, hi) if p == "high" else max(lo, hi) for p in MT_SIDE_PRIORITY)
-        s = _MT_SIDE[device.index] = (torch.cuda.Stream(device, priority=pj),
-                                      [torch.cuda.Stream(device, priority=pg) for _ in range(MT_MAX_SLOTS)])
+        s = _MT_SIDE[device.index] = (torch.cuda.Stream(device),
+                                      [torch.cuda.Stream(device) for _ in range(MT_MAX_SLOTS)])
     return s
 
 
@@ -1329,7 +1328,7 @@ def mt19937_reserve(count: int, device, fmt: str = "plain"):
     bits tie (about 1 draw in 2^8 / 2^16).  A request the run cannot honour
     gets plain draws.
 
-    The draws are generated on two high-priority side streams
+    The draws are generated on two side streams
     (gc_mt19937_generate_split_j): phase 1 (jump stream) = the state's
     sequence, the LDS-bound jumps and one more jump straight to the END state;
     phase 2 (generator stream) = the latency-bound generators.  The host waits
