@@ -1,0 +1,909 @@
+// grad_clip.hip — the global norm of many gradient tensors and the clipping
+// that follows it (include/gcodec.h gc_grad_*, gc_qsgd_decode_clip).
+//
+//   N = (sum_t sum_i |x_ti|^p)^(1/p),  p = 1, 2 or infinity (N = max |x|)
+//   c = min(1, max_norm / (N + 1e-6)),  y = RN_type(x c)
+//
+// Two passes, and nothing is kept between calls: k_grad_norm (or k_lane_norm,
+// from packed words) leaves one partial a block in the caller's workspace, and
+// every wave of the pass that writes (k_grad_scale, k_decode_clip) adds those
+// partials in one fixed order and forms c itself.  So there are no atomics, no
+// tickets and no zeroed state: the result does not depend on the schedule, a
+// captured call owns all that it writes, and two calls on different streams
+// share nothing.
+//
+// Sums are held in 64 bits: the square of a float32 is exact to half an ulp
+// there and cannot overflow or vanish, so N is right for any gradients whose
+// norm a float32 can hold (1e-45 .. 3e38) and c even beyond.  One conversion
+// and one fused multiply-add for each element are about a seventh of the
+// vector unit's time at the rate that the memory delivers float32.
+//
+// All of it is bound by HBM: norm reads the gradients once; clip reads them
+// twice and writes them once, the second read walking backwards so that what
+// the first read last is still in the 256 MB of cache in front of the memory.
+#include "gc_device.h"
+#include "gc_host.h"
+#include "grads.h"
+
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+namespace gc {
+
+constexpr uint32_t kTile = 2048;       // flat elements a wave takes at a time
+constexpr unsigned kNormThreads = 1024;
+constexpr unsigned kNormGrid = 512;    // two blocks a CU: 32 waves, each with 4 KB in flight
+constexpr unsigned kScaleThreads = 256;
+constexpr unsigned kScaleGrid = 2048;
+constexpr double kEps = 1e-6;
+
+// workspace: kNormGrid partials (64-bit), kNormGrid maxima (32-bit), then the
+// pieces' sums of the per-tensor norms
+constexpr size_t kWsPeak = kNormGrid * 8;
+constexpr size_t kWsSlots = kWsPeak + kNormGrid * 4;
+
+// p as the kernels' template argument; kPInf sums by maximum
+constexpr int kPInf = 0;
+
+// ---------------------------------------------------------------------------
+// accumulation
+// ---------------------------------------------------------------------------
+// An accumulator of |x|^p.  p = infinity keeps the bits of |x| as an integer:
+// their order is the values' order, and a NaN is above them all and stays.
+template <int P>
+struct Acc {
+    double v = 0.0;
+    __device__ __forceinline__ void add(float x)
+    {
+        const double d = (double)x;
+        v = P == 2 ? fma(d, d, v) : v + fabs(d);
+    }
+    __device__ __forceinline__ void join(const Acc &o) { v += o.v; }
+    __device__ __forceinline__ Acc shuffled(int m) const
+    {
+        Acc r;
+        r.v = __shfl_xor(v, m, 64);
+        return r;
+    }
+    __device__ __forceinline__ double value() const { return v; }
+    __device__ __forceinline__ void set(double x) { v = x; }
+};
+template <>
+struct Acc<kPInf> {
+    uint32_t m = 0;
+    __device__ __forceinline__ void add(float x) { m = max(m, __float_as_uint(x) & 0x7fffffffu); }
+    __device__ __forceinline__ void join(const Acc &o) { m = max(m, o.m); }
+    __device__ __forceinline__ Acc shuffled(int k) const
+    {
+        Acc r;
+        r.m = (uint32_t)__shfl_xor((int)m, k, 64);
+        return r;
+    }
+    __device__ __forceinline__ double value() const { return (double)__uint_as_float(m); }
+    __device__ __forceinline__ void set(double x) { m = __float_as_uint((float)x); }  // a float's own value back
+};
+
+template <class A>
+__device__ __forceinline__ void wave_join(A &a)
+{
+#pragma unroll
+    for (int m = 32; m; m >>= 1)
+        a.join(a.shuffled(m));
+}
+
+// the wave's elements x[0 .. cnt), x and cnt the same for all lanes
+template <class T, class F>
+__device__ __forceinline__ void wave_read(Glob<const T> x, uint32_t cnt, F f)
+{
+    constexpr uint32_t V = 16 / sizeof(T), step = 64 * V, U = 4;
+    const uint32_t lane = lane_id();
+    uint32_t i = 0;
+    for (; i + U * step <= cnt; i += U * step) {
+        typename VecOf<T, V>::type v[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            v[u] = ldv<T, V>(x + i + u * step + lane * V);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+            for (uint32_t k = 0; k < V; ++k)
+                f(Elem<T>::up(v[u][k]));
+    }
+    for (; i < cnt; i += step) {
+        const uint32_t j = i + lane * V;
+        if (j + V <= cnt) {
+            const auto v = ldv<T, V>(x + j);
+#pragma unroll
+            for (uint32_t k = 0; k < V; ++k)
+                f(Elem<T>::up(v[k]));
+        } else {
+            for (uint32_t k = j; k < cnt; ++k)
+                f(Elem<T>::up(x[k]));
+        }
+    }
+}
+
+template <class F>
+__device__ __forceinline__ void wave_read_any(uint32_t type, uint64_t base, uint64_t off, uint32_t cnt, F f)
+{
+    if (type == kTF32)
+        wave_read<float>(glob<const float>(base, off), cnt, f);
+    else if (type == kTBF16)
+        wave_read<__bf16>(glob<const __bf16>(base, off), cnt, f);
+    else
+        wave_read<_Float16>(glob<const _Float16>(base, off), cnt, f);
+}
+
+// One partial of |x|^p a block (and, PEAK, one of max |x|).  EACH: also the sum
+// of every piece, at slot (tile + tensor): along the flat sequence each next
+// piece has the next tile or the next tensor, so a tensor's pieces have
+// consecutive slots of their own.
+template <int P, bool EACH, bool PEAK, bool LDS>
+__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, double *__restrict__ part,
+                                                            uint32_t *__restrict__ peak, double *__restrict__ slots)
+{
+    __shared__ GradRec srec[LDS ? kLdsRecs + 1 : 1];
+    __shared__ double sacc[kNormThreads / 64];
+    __shared__ uint32_t smax[kNormThreads / 64];
+    const GradRec *rec = LDS ? srec : g.rec;
+    if (LDS && n) {
+        stage_table(g, srec);
+        __syncthreads();
+    }
+    Acc<P> all;
+    Acc<kPInf> top;
+    const uint64_t tiles = (n + kTile - 1) / kTile, waves = (uint64_t)gridDim.x * (kNormThreads / 64);
+    for (uint64_t t = (uint64_t)blockIdx.x * (kNormThreads / 64) + wave_id(); t < tiles; t += waves) {
+        const uint64_t lo = t * kTile, hi = min(lo + kTile, n);
+        grad_walk(rec, g.count, lo, hi,
+                  [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
+                      Acc<P> one;
+                      Acc<P> &acc = EACH ? one : all;
+                      wave_read_any(type, base, a - start, (uint32_t)(b - a), [&](float x) {
+                          acc.add(x);
+                          if (PEAK)
+                              top.add(x);
+                      });
+                      if (EACH) {
+                          all.join(one);
+                          wave_join(one);
+                          if (lane_id() == 0)
+                              slots[t + s] = one.value();
+                      }
+                  });
+    }
+    wave_join(all);
+    if (PEAK)
+        wave_join(top);
+    if (lane_id() == 0) {
+        sacc[wave_id()] = all.value();
+        if (PEAK)
+            smax[wave_id()] = top.m;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (unsigned w = 1; w < kNormThreads / 64; ++w) {
+            Acc<P> o;
+            o.set(sacc[w]);
+            all.join(o);
+            if (PEAK)
+                top.m = max(top.m, smax[w]);
+        }
+        part[blockIdx.x] = all.value();
+        if (PEAK)
+            peak[blockIdx.x] = top.m;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// finish: the partials in one fixed order, by every wave that needs them
+// ---------------------------------------------------------------------------
+template <int P>
+__device__ __forceinline__ double wave_total(const double *__restrict__ part, uint32_t parts)
+{
+    Acc<P> a;
+    for (uint32_t i = lane_id(); i < parts; i += 64) {
+        Acc<P> o;
+        o.set(part[i]);
+        a.join(o);
+    }
+    wave_join(a);
+    return a.value();
+}
+
+__device__ __forceinline__ double wave_total_of(int p, const double *part, uint32_t parts)
+{
+    return p == 2 ? wave_total<2>(part, parts) : p == 1 ? wave_total<1>(part, parts) : wave_total<kPInf>(part, parts);
+}
+
+__device__ __forceinline__ double root_of(int p, double total) { return p == 2 ? sqrt(total) : total; }
+
+// min(1, max_norm / (N + 1e-6)); a NaN stays one, as in torch's clamp
+__device__ __forceinline__ float clip_coef(double norm, double max_norm)
+{
+    const double q = max_norm / (norm + kEps);
+    return q > 1.0 ? 1.0f : (float)q;
+}
+
+// block 0: the total and N; block 1 + s (EACH): the norm of tensor s
+__global__ __launch_bounds__(kScaleThreads) void k_grad_finish(GradArg g, int p, const double *__restrict__ part,
+                                                               uint32_t parts, const double *__restrict__ slots,
+                                                               double *__restrict__ total, float *__restrict__ norm,
+                                                               float *__restrict__ each)
+{
+    if (blockIdx.x == 0) {
+        if (wave_id() == 0) {
+            const double t = wave_total_of(p, part, parts);
+            if (lane_id() == 0) {
+                if (total)
+                    *total = t;
+                if (norm)
+                    *norm = (float)root_of(p, t);
+            }
+        }
+        return;
+    }
+    __shared__ double sw[kScaleThreads / 64];
+    const uint32_t s = blockIdx.x - 1;
+    const uint64_t a = g.rec[s].start, b = g.rec[s + 1].start;
+    if (a == b) {
+        if (threadIdx.x == 0)
+            each[s] = 0.0f;
+        return;
+    }
+    // the same number of slots for every wave's share, then the waves in order
+    const uint64_t s0 = a / kTile + s, cnt = (b - 1) / kTile + s + 1 - s0;
+    const uint64_t share = (cnt + kScaleThreads / 64 - 1) / (kScaleThreads / 64), w0 = wave_id() * share;
+    const uint64_t mine = w0 < cnt ? min(share, cnt - w0) : 0;
+    const double t = wave_total_of(p, slots + s0 + w0, (uint32_t)mine);
+    if (lane_id() == 0)
+        sw[wave_id()] = t;
+    __syncthreads();
+    if (wave_id() == 0) {
+        const double r = wave_total_of(p, sw, kScaleThreads / 64);
+        if (lane_id() == 0)
+            each[s] = (float)root_of(p, r);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// scale
+// ---------------------------------------------------------------------------
+template <class TS, class TD>
+__device__ __forceinline__ void wave_scale(Glob<const TS> x, Glob<TD> y, uint32_t cnt, float c)
+{
+    constexpr uint32_t V = sizeof(TS) == 2 && sizeof(TD) == 2 ? 8 : 4, step = 64 * V, U = 4;
+    const uint32_t lane = lane_id();
+    uint32_t i = 0;
+    for (; i + U * step <= cnt; i += U * step) {
+        typename VecOf<TS, V>::type v[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            v[u] = ldv<TS, V>(x + i + u * step + lane * V);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            float f[V];
+#pragma unroll
+            for (uint32_t k = 0; k < V; ++k)
+                f[k] = Elem<TS>::up(v[u][k]) * c;
+            stv<TD, V>(y + i + u * step + lane * V, f);
+        }
+    }
+    for (; i < cnt; i += step) {
+        const uint32_t j = i + lane * V;
+        if (j + V <= cnt) {
+            const auto v = ldv<TS, V>(x + j);
+            float f[V];
+#pragma unroll
+            for (uint32_t k = 0; k < V; ++k)
+                f[k] = Elem<TS>::up(v[k]) * c;
+            stv<TD, V>(y + j, f);
+        } else {
+            for (uint32_t k = j; k < cnt; ++k)
+                y[k] = Elem<TD>::down(Elem<TS>::up(x[k]) * c);
+        }
+    }
+}
+
+template <class TS>
+__device__ __forceinline__ void wave_scale_to(uint32_t td, Glob<const TS> x, uint64_t base, uint64_t off, uint32_t cnt,
+                                              float c)
+{
+    if (td == kTF32)
+        wave_scale<TS, float>(x, glob<float>(base, off), cnt, c);
+    else if (td == kTBF16)
+        wave_scale<TS, __bf16>(x, glob<__bf16>(base, off), cnt, c);
+    else
+        wave_scale<TS, _Float16>(x, glob<_Float16>(base, off), cnt, c);
+}
+
+// y = RN(x c) from the tensors of src into those of dst (the same sizes), or
+// (FLAT) end to end into float32.  The partials' pass has c = 1 in most steps
+// of a training run; in place nothing is left to do then.
+template <bool FLAT, bool LDS>
+__global__ __launch_bounds__(kScaleThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n, int p,
+                                                              double max_norm, const double *__restrict__ part,
+                                                              uint32_t parts, const uint32_t *__restrict__ peaks,
+                                                              bool in_place, float *__restrict__ norm,
+                                                              float *__restrict__ peak)
+{
+    const double N = root_of(p, wave_total_of(p, part, parts));
+    const float c = clip_coef(N, max_norm);
+    if (blockIdx.x == 0 && wave_id() == 0) {
+        if (FLAT) {
+            // max |RN(x c)| = RN(max |x| c): rounding keeps the order.  A NaN
+            // or infinite x with c = NaN or 0 gives NaN on both sides.
+            Acc<kPInf> top;
+            for (uint32_t i = lane_id(); i < parts; i += 64)
+                top.m = max(top.m, peaks[i]);
+            wave_join(top);
+            if (lane_id() == 0)
+                *peak = __uint_as_float(top.m) * c;
+        }
+        if (norm && lane_id() == 0)
+            *norm = (float)N;
+    }
+    if (in_place && c == 1.0f)
+        return;
+    __shared__ GradRec ss[LDS ? kLdsRecs + 1 : 1];
+    __shared__ GradRec sd[LDS && !FLAT ? kLdsRecs + 1 : 1];
+    const GradRec *rs = LDS ? ss : src.rec, *rd = LDS ? sd : dst.rec;
+    if (LDS && n) {
+        stage_table(src, ss);
+        if (!FLAT)
+            stage_table(dst, sd);
+        __syncthreads();
+    }
+    const uint64_t tiles = (n + kTile - 1) / kTile, waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
+    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves) {
+        const uint64_t lo = (tiles - 1 - t) * kTile, hi = min(lo + kTile, n);
+        grad_walk(rs, src.count, lo, hi,
+                  [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
+                      const uint64_t dpt = FLAT ? (uint64_t)kTF32 << 56 | reinterpret_cast<uint64_t>(flat) : uni64(rd[s].pt);
+                      const uint64_t off = a - start, doff = FLAT ? a : off;
+                      const uint32_t td = (uint32_t)(dpt >> 56), cnt = (uint32_t)(b - a);
+                      const uint64_t dbase = dpt & 0x00ffffffffffffffull;
+                      if (type == kTF32)
+                          wave_scale_to<float>(td, glob<const float>(base, off), dbase, doff, cnt, c);
+                      else if (type == kTBF16)
+                          wave_scale_to<__bf16>(td, glob<const __bf16>(base, off), dbase, doff, cnt, c);
+                      else
+                          wave_scale_to<_Float16>(td, glob<const _Float16>(base, off), dbase, doff, cnt, c);
+                  });
+    }
+}
+
+// ---------------------------------------------------------------------------
+// decode: v = RN(RN(k Q) alpha), k = RN(norm / s), Q = lane - W s (k_qsgd_decode's
+// arithmetic), the norm of the v, and y = RN_type(RN(v c))
+// ---------------------------------------------------------------------------
+struct LaneArg {
+    const uint32_t *words;
+    uint64_t n, M;
+    const float *norm;
+    float s, alpha;
+    int32_t sub;   // W s
+    uint32_t w;    // lane width
+    uint32_t L;    // lanes a word
+    uint32_t qmax; // largest |Q|
+};
+
+// v depends on Q alone, so the norm is |k alpha| times the norm of the
+// integers, whose sum is exact in any order.  Where that product is not the
+// sum of the rounded v to within their own roundings (values that overflow or
+// fall below the normal range, wide lanes whose squares pass 32 bits), the
+// values themselves are added in 64 bits.
+__device__ __forceinline__ bool lanes_exact(const LaneArg &a, float k)
+{
+    const double step = fabs((double)k * (double)a.alpha), top = fabs((double)k) * (double)a.qmax;
+    return a.w <= 14 && step >= 1e-30 && step <= 1e30 && top <= 1e38 && top * fabs((double)a.alpha) <= 1e38;
+}
+
+template <int P>
+__device__ __forceinline__ double lanes_norm(const LaneArg &a, float k, const uint64_t *__restrict__ part, uint32_t parts)
+{
+    if (lanes_exact(a, k)) {
+        uint64_t t = 0;
+        for (uint32_t i = lane_id(); i < parts; i += 64)
+            t = P == kPInf ? max(t, part[i]) : t + part[i];
+#pragma unroll
+        for (int m = 32; m; m >>= 1) {
+            const uint64_t o = __shfl_xor(t, m, 64);
+            t = P == kPInf ? max(t, o) : t + o;
+        }
+        if (P == kPInf)
+            return fabs((double)(k * (float)t * a.alpha));
+        const double step = fabs((double)k * (double)a.alpha);
+        return P == 2 ? step * sqrt((double)t) : step * (double)t;
+    }
+    return root_of(P, wave_total<P>(reinterpret_cast<const double *>(part), parts));
+}
+
+template <int P>
+__global__ __launch_bounds__(kNormThreads) void k_lane_norm(LaneArg a, uint64_t *__restrict__ part)
+{
+    __shared__ uint64_t sint[kNormThreads / 64];
+    const float k = *a.norm / a.s;
+    const bool exact = lanes_exact(a, k);
+    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u;
+    const uint64_t quads = a.M >> 2, stride = (uint64_t)gridDim.x * kNormThreads;
+    uint64_t sum = 0;
+    Acc<P> real;
+    for (uint64_t t = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x; t < quads; t += stride) {
+        const uint4 wd = *reinterpret_cast<const uint4 *>(a.words + 4 * t);
+        uint32_t we[4] = {wd.x, wd.y, wd.z, wd.w};
+        uint32_t quad = 0;  // w <= 14: at most L * 4 * 2^(2w) <= 2^31
+        for (uint32_t l = 0; l < a.L; ++l) {
+            const uint64_t i0 = (uint64_t)l * a.M + 4 * t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int32_t q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
+                const bool in = i0 + e < a.n;
+                if (exact) {
+                    const uint32_t m = in ? (uint32_t)(q < 0 ? -q : q) : 0u;
+                    quad = P == kPInf ? max(quad, m) : P == 2 ? quad + m * m : quad + m;
+                } else if (in) {
+                    real.add(k * (float)q * a.alpha);
+                }
+            }
+        }
+        sum = P == kPInf ? max(sum, (uint64_t)quad) : sum + quad;
+    }
+    if (exact) {
+#pragma unroll
+        for (int m = 32; m; m >>= 1) {
+            const uint64_t o = __shfl_xor(sum, m, 64);
+            sum = P == kPInf ? max(sum, o) : sum + o;
+        }
+    } else {
+        wave_join(real);
+        sum = (uint64_t)__double_as_longlong(real.value());
+    }
+    if (lane_id() == 0)
+        sint[wave_id()] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (unsigned w = 1; w < kNormThreads / 64; ++w) {
+            if (exact) {
+                sum = P == kPInf ? max(sum, sint[w]) : sum + sint[w];
+            } else {
+                Acc<P> o;
+                o.set(__longlong_as_double((long long)sint[w]));
+                real.join(o);
+            }
+        }
+        part[blockIdx.x] = exact ? sum : (uint64_t)__double_as_longlong(real.value());
+    }
+}
+
+// the lane's quad v of flat elements i .. i + 3, those inside [a, b), to the
+// tensor at base whose first element is start
+template <class T>
+__device__ __forceinline__ void store_quad(uint64_t base, uint64_t start, uint64_t a, uint64_t b, uint64_t i, const float (&v)[4])
+{
+    const Glob<T> y = glob<T>(base, 0);
+    if (i >= a && i + 4 <= b) {
+        stv<T, 4>(y + (i - start), v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e >= a && i + e < b)
+            y[i + e - start] = Elem<T>::down(v[e]);
+}
+
+// A wave takes 256 kQuads consecutive words, L ranges of as many flat elements
+template <bool LDS>
+__global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradArg dst, int p, double max_norm,
+                                                               const uint64_t *__restrict__ part, uint32_t parts,
+                                                               float *__restrict__ norm)
+{
+    constexpr int kQuads = 2;
+    const float k = *a.norm / a.s;
+    const double N = p == 2   ? lanes_norm<2>(a, k, part, parts)
+                     : p == 1 ? lanes_norm<1>(a, k, part, parts)
+                              : lanes_norm<kPInf>(a, k, part, parts);
+    const float c = clip_coef(N, max_norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *norm = (float)N;
+    __shared__ GradRec sd[LDS ? kLdsRecs + 1 : 1];
+    const GradRec *rd = LDS ? sd : dst.rec;
+    if (LDS && a.n) {
+        stage_table(dst, sd);
+        __syncthreads();
+    }
+    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u, lane = lane_id();
+    const uint64_t tiles = (a.M + 256 * kQuads - 1) / (256 * kQuads), waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
+    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves) {
+        const uint64_t j0 = t * (256 * kQuads), j1 = min(j0 + 256 * kQuads, a.M);
+        uint4 wd[kQuads];
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+            const uint64_t j = j0 + 256 * q + 4 * lane;  // M is a multiple of 4: a quad is in or out
+            wd[q] = j < j1 ? *reinterpret_cast<const uint4 *>(a.words + j) : make_uint4(0, 0, 0, 0);
+        }
+        for (uint32_t l = 0; l < a.L; ++l) {
+            const uint64_t lo = (uint64_t)l * a.M + j0, hi = min((uint64_t)l * a.M + j1, a.n);
+            if (lo >= hi)
+                break;
+            grad_walk(rd, dst.count, lo, hi,
+                      [&](uint32_t, uint32_t type, uint64_t base, uint64_t start, uint64_t pa, uint64_t pb) {
+#pragma unroll
+                          for (int q = 0; q < kQuads; ++q) {
+                              if (lo + 256 * q >= pb || lo + 256 * (q + 1) <= pa)
+                                  continue;
+                              const uint32_t we[4] = {wd[q].x, wd[q].y, wd[q].z, wd[q].w};
+                              float v[4];
+#pragma unroll
+                              for (int e = 0; e < 4; ++e) {
+                                  const int32_t Q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
+                                  const float d = k * (float)Q;
+                                  v[e] = d * a.alpha * c;
+                              }
+                              const uint64_t i = lo + 256 * q + 4 * lane;
+                              if (type == kTF32)
+                                  store_quad<float>(base, start, pa, pb, i, v);
+                              else if (type == kTBF16)
+                                  store_quad<__bf16>(base, start, pa, pb, i, v);
+                              else
+                                  store_quad<_Float16>(base, start, pa, pb, i, v);
+                          }
+                      });
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// table
+// ---------------------------------------------------------------------------
+constexpr uint32_t kFillRecs = 224;  // records a launch carries in its arguments (3.5 KB)
+struct FillArg {
+    GradRec rec[kFillRecs];
+};
+
+__global__ __launch_bounds__(256) void k_grads_fill(FillArg a, uint32_t cnt, GradRec *__restrict__ out)
+{
+    if (threadIdx.x < cnt)
+        out[threadIdx.x] = a.rec[threadIdx.x];
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+static size_t elem_size(uint64_t pt) { return (pt >> 56) == kTF32 ? 4 : 2; }
+
+struct Span {  // a tensor's bytes
+    uint64_t lo, hi;
+};
+static Span span_of(const gc_grads *g, uint64_t s)
+{
+    const uint64_t pt = g->host_rec[2 * s], lo = pt & 0x00ffffffffffffffull;
+    return {lo, lo + (g->host_rec[2 * s + 3] - g->host_rec[2 * s + 1]) * elem_size(pt)};
+}
+
+static int check_grads(const gc_grads *g, const char *what)
+{
+    GC_REQUIRE(g, "%s: null gradient table", what);
+    GC_REQUIRE(g->count < (1ull << 31), "%s: more than 2^31 tensors", what);
+    GC_REQUIRE(g->host_rec && g->order, "%s: gradient table without its host image", what);
+    GC_REQUIRE(g->host_rec[2 * g->count + 1] == g->n, "%s: gradient table's host image does not end at n", what);
+    GC_REQUIRE(g->count == 0 || g->rec, "%s: gradient table not on the device", what);
+    return GC_OK;
+}
+
+static int check_output(const gc_grads *g, const char *what)
+{
+    GC_REQUIRE(!(g->flags & GC_GRADS_OVERLAP), "%s: tensors to be written share memory", what);
+    return GC_OK;
+}
+
+// whether [lo, hi) meets a tensor of the (disjoint) table; *at its index
+static bool meets(const gc_grads *g, Span x, uint64_t *at)
+{
+    if (x.lo >= x.hi)
+        return false;
+    uint64_t a = 0, b = g->count;  // order[]: non-empty tensors by address, then the empty ones
+    while (a < b) {
+        const uint64_t m = (a + b) / 2;
+        const Span y = span_of(g, g->order[m]);
+        if (y.lo < y.hi && y.hi <= x.lo)
+            a = m + 1;
+        else
+            b = m;
+    }
+    if (a == g->count)
+        return false;
+    const Span y = span_of(g, g->order[a]);
+    *at = g->order[a];
+    return y.lo < y.hi && y.lo < x.hi;
+}
+
+static int check_p(uint32_t p, const char *what)
+{
+    GC_REQUIRE(p == 1 || p == 2 || p == GC_NORM_INF, "%s: the norm is GC_NORM_INF, 1 or 2, got %u", what, p);
+    return GC_OK;
+}
+
+static int check_max_norm(double m, const char *what)
+{
+    GC_REQUIRE(m >= 0.0, "%s: max_norm %g is not a number at or above 0", what, m);
+    return GC_OK;
+}
+
+static GradArg arg_of(const gc_grads *g)
+{
+    return {reinterpret_cast<const GradRec *>(g->rec), (uint32_t)g->count};
+}
+
+static unsigned norm_grid(uint64_t n)
+{
+    const uint64_t tiles = (n + kTile - 1) / kTile, per = kNormThreads / 64;
+    return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
+}
+
+// the partials of the norm -> their number
+template <bool EACH, bool PEAK>
+static void launch_norm(const gc_grads *g, uint32_t p, void *ws, hipStream_t st)
+{
+    const GradArg a = arg_of(g);
+    const unsigned grid = norm_grid(g->n);
+    char *w = static_cast<char *>(ws);
+    double *part = reinterpret_cast<double *>(w);
+    uint32_t *peak = reinterpret_cast<uint32_t *>(w + kWsPeak);
+    double *slots = reinterpret_cast<double *>(w + kWsSlots);
+    const bool lds = g->count <= kLdsRecs;
+#define GC_GN(P_)                                                                                                   \
+    do {                                                                                                            \
+        if (lds)                                                                                                    \
+            hipLaunchKernelGGL((k_grad_norm<P_, EACH, PEAK, true>), dim3(grid), dim3(kNormThreads), 0, st, a, g->n, \
+                               part, peak, slots);                                                                  \
+        else                                                                                                        \
+            hipLaunchKernelGGL((k_grad_norm<P_, EACH, PEAK, false>), dim3(grid), dim3(kNormThreads), 0, st, a,      \
+                               g->n, part, peak, slots);                                                            \
+    } while (0)
+    if (p == 2)
+        GC_GN(2);
+    else if (p == 1)
+        GC_GN(1);
+    else
+        GC_GN(kPInf);
+#undef GC_GN
+}
+
+static unsigned scale_grid(uint64_t tiles)
+{
+    const uint64_t per = kScaleThreads / 64;
+    return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kScaleGrid);
+}
+
+}  // namespace gc
+
+using namespace gc;
+
+static_assert(sizeof(GradRec) == 16, "gc_grads.rec layout");
+
+extern "C" {
+
+int gc_grads_plan(const uint64_t *sizes, const void *const *ptrs, const uint32_t *types, uint64_t count,
+                  uint64_t *rec, uint32_t *order, gc_grads *out)
+{
+    const char *what = "gc_grads_plan";
+    GC_REQUIRE(out && rec && order, "%s: null output", what);
+    GC_REQUIRE(count == 0 || (sizes && ptrs && types), "%s: null input", what);
+    GC_REQUIRE(count < (1ull << 31), "%s: more than 2^31 tensors", what);
+    uint64_t n = 0;
+    for (uint64_t s = 0; s < count; ++s) {
+        GC_REQUIRE(types[s] == GC_F32 || types[s] == GC_F16 || types[s] == GC_BF16,
+                   "%s: tensor %llu is not float32, float16 or bfloat16", what, (unsigned long long)s);
+        const uint64_t at = reinterpret_cast<uint64_t>(ptrs[s]), size = types[s] == GC_F32 ? 4 : 2;
+        GC_REQUIRE(sizes[s] == 0 || ptrs[s], "%s: tensor %llu has no data pointer", what, (unsigned long long)s);
+        GC_REQUIRE(at % size == 0 && at >> 56 == 0, "%s: tensor %llu is not aligned to its elements", what,
+                   (unsigned long long)s);
+        GC_REQUIRE(sizes[s] < (1ull << 52) && n + sizes[s] < (1ull << 52), "%s: size overflow", what);
+        const uint64_t tag = types[s] == GC_F32 ? kTF32 : types[s] == GC_F16 ? kTF16 : kTBF16;
+        rec[2 * s] = tag << 56 | at;
+        rec[2 * s + 1] = n;
+        n += sizes[s];
+        order[s] = (uint32_t)s;
+    }
+    rec[2 * count] = 0;
+    rec[2 * count + 1] = n;
+    gc_grads g{};
+    g.count = count;
+    g.n = n;
+    g.host_rec = rec;
+    g.order = order;
+    std::sort(order, order + count, [&](uint32_t x, uint32_t y) {
+        const Span a = span_of(&g, x), b = span_of(&g, y);
+        const bool ea = a.lo == a.hi, eb = b.lo == b.hi;
+        if (ea != eb)
+            return eb;
+        return ea ? x < y : a.lo != b.lo ? a.lo < b.lo : x < y;
+    });
+    uint64_t end = 0;
+    for (uint64_t i = 0; i < count; ++i) {
+        const Span a = span_of(&g, order[i]);
+        if (a.lo == a.hi)
+            break;
+        if (a.lo < end)
+            g.flags |= GC_GRADS_OVERLAP;
+        end = std::max(end, a.hi);
+    }
+    *out = g;
+    return GC_OK;
+}
+
+int gc_grads_fill(const gc_grads *grads, uint64_t *rec, gc_stream_t stream)
+{
+    const char *what = "gc_grads_fill";
+    GC_REQUIRE(grads && grads->host_rec && rec, "%s: null pointer", what);
+    const GradRec *h = reinterpret_cast<const GradRec *>(grads->host_rec);
+    GradRec *d = reinterpret_cast<GradRec *>(rec);
+    for (uint64_t i = 0; i <= grads->count; i += kFillRecs) {
+        const uint32_t cnt = (uint32_t)std::min<uint64_t>(kFillRecs, grads->count + 1 - i);
+        FillArg a;
+        std::copy(h + i, h + i + cnt, a.rec);
+        std::fill(a.rec + cnt, a.rec + kFillRecs, GradRec{0, 0});
+        hipLaunchKernelGGL(k_grads_fill, dim3(1), dim3(256), 0, as_stream(stream), a, cnt, d + i);
+    }
+    return launch_status(what);
+}
+
+size_t gc_grad_workspace_size(uint64_t n, uint64_t count, int each)
+{
+    return kWsSlots + (each ? ((n + kTile - 1) / kTile + count) * sizeof(double) : 0);
+}
+
+int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, float *each, void *workspace,
+                 gc_stream_t stream)
+{
+    const char *what = "gc_grad_norm";
+    int rc;
+    if ((rc = check_grads(grads, what)) || (rc = check_p(p, what)))
+        return rc;
+    GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
+    hipStream_t st = as_stream(stream);
+    if (each)
+        launch_norm<true, false>(grads, p, workspace, st);
+    else
+        launch_norm<false, false>(grads, p, workspace, st);
+    char *w = static_cast<char *>(workspace);
+    const unsigned blocks = 1 + (each ? (unsigned)grads->count : 0u);
+    hipLaunchKernelGGL(k_grad_finish, dim3(blocks), dim3(kScaleThreads), 0, st, arg_of(grads), (int)p,
+                       reinterpret_cast<const double *>(w), norm_grid(grads->n),
+                       reinterpret_cast<const double *>(w + kWsSlots), total, norm, each);
+    return launch_status(what);
+}
+
+int gc_grad_norm_root(const double *total, uint32_t p, float *norm, gc_stream_t stream)
+{
+    const char *what = "gc_grad_norm_root";
+    int rc;
+    if ((rc = check_p(p, what)))
+        return rc;
+    GC_REQUIRE(total && norm, "%s: null pointer", what);
+    hipLaunchKernelGGL(k_grad_finish, dim3(1), dim3(kScaleThreads), 0, as_stream(stream), GradArg{nullptr, 0}, (int)p,
+                       total, 1u, nullptr, nullptr, norm, nullptr);
+    return launch_status(what);
+}
+
+int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double max_norm, const double *total,
+                 float *norm, void *workspace, gc_stream_t stream)
+{
+    const char *what = "gc_grad_clip";
+    int rc;
+    if ((rc = check_grads(src, what)) || (rc = check_grads(dst, what)) || (rc = check_output(dst, what)) ||
+        (rc = check_p(p, what)) || (rc = check_max_norm(max_norm, what)))
+        return rc;
+    GC_REQUIRE(src->count == dst->count, "%s: %llu tensors into %llu", what, (unsigned long long)src->count,
+               (unsigned long long)dst->count);
+    bool same = true;
+    for (uint64_t s = 0; s <= src->count; ++s) {
+        GC_REQUIRE(src->host_rec[2 * s + 1] == dst->host_rec[2 * s + 1], "%s: the two lists differ in tensor sizes", what);
+        same &= src->host_rec[2 * s] == dst->host_rec[2 * s];
+    }
+    for (uint64_t s = 0; !same && s < src->count; ++s) {
+        uint64_t at = 0;
+        const Span x = span_of(src, s);
+        // a tensor may be clipped onto itself; any other meeting would be read after it is written
+        if (meets(dst, x, &at))
+            GC_REQUIRE(at == s && src->host_rec[2 * s] == dst->host_rec[2 * s],
+                       "%s: input tensor %llu shares memory with output tensor %llu", what, (unsigned long long)s,
+                       (unsigned long long)at);
+    }
+    GC_REQUIRE(total || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0),
+               "%s: null or misaligned workspace", what);
+    hipStream_t st = as_stream(stream);
+    if (!total)
+        launch_norm<false, false>(src, p, workspace, st);
+    const double *part = total ? total : static_cast<const double *>(workspace);
+    const unsigned parts = total ? 1u : norm_grid(src->n);
+    const unsigned grid = scale_grid((src->n + kTile - 1) / kTile);
+    const GradArg a = arg_of(src), b = arg_of(dst);
+    if (src->count <= kLdsRecs)
+        hipLaunchKernelGGL((k_grad_scale<false, true>), dim3(grid), dim3(kScaleThreads), 0, st, a, b, nullptr, src->n,
+                           (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
+    else
+        hipLaunchKernelGGL((k_grad_scale<false, false>), dim3(grid), dim3(kScaleThreads), 0, st, a, b, nullptr, src->n,
+                           (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
+    return launch_status(what);
+}
+
+int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double max_norm, float *peak, float *norm,
+                         void *workspace, gc_stream_t stream)
+{
+    const char *what = "gc_grad_flatten_clip";
+    int rc;
+    if ((rc = check_grads(src, what)) || (rc = check_p(p, what)) || (rc = check_max_norm(max_norm, what)))
+        return rc;
+    GC_REQUIRE(peak && (src->n == 0 || flat) && (reinterpret_cast<uintptr_t>(flat) & 3u) == 0,
+               "%s: null or misaligned output", what);
+    GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
+    const uint64_t lo = reinterpret_cast<uint64_t>(flat), hi = lo + 4 * src->n;
+    for (uint64_t s = 0; s < src->count; ++s) {
+        const Span x = span_of(src, s);
+        GC_REQUIRE(x.lo >= x.hi || x.hi <= lo || x.lo >= hi, "%s: input tensor %llu lies in the flat bucket", what,
+                   (unsigned long long)s);
+    }
+    hipStream_t st = as_stream(stream);
+    launch_norm<false, true>(src, p, workspace, st);
+    const char *w = static_cast<const char *>(workspace);
+    const unsigned grid = scale_grid((src->n + kTile - 1) / kTile), parts = norm_grid(src->n);
+    const GradArg a = arg_of(src);
+    const double *part = reinterpret_cast<const double *>(w);
+    const uint32_t *peaks = reinterpret_cast<const uint32_t *>(w + kWsPeak);
+    if (src->count <= kLdsRecs)
+        hipLaunchKernelGGL((k_grad_scale<true, true>), dim3(grid), dim3(kScaleThreads), 0, st, a, GradArg{}, flat, src->n,
+                           (int)p, max_norm, part, parts, peaks, false, norm, peak);
+    else
+        hipLaunchKernelGGL((k_grad_scale<true, false>), dim3(grid), dim3(kScaleThreads), 0, st, a, GradArg{}, flat, src->n,
+                           (int)p, max_norm, part, parts, peaks, false, norm, peak);
+    return launch_status(what);
+}
+
+int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, uint32_t bits, const gc_lanes *lanes,
+                        float alpha, const gc_grads *dst, uint32_t p, double max_norm, float *total_norm,
+                        void *workspace, gc_stream_t stream)
+{
+    const char *what = "gc_qsgd_decode_clip";
+    int rc;
+    if ((rc = check_bits(bits, what)) || (rc = check_lanes(lanes, n, what)) || (rc = check_grads(dst, what)) ||
+        (rc = check_output(dst, what)) || (rc = check_p(p, what)) || (rc = check_max_norm(max_norm, what)))
+        return rc;
+    const uint32_t s = (1u << bits) - 1u;
+    GC_REQUIRE(lanes->offset == s && lanes->range == 2ull * s, "%s: lanes not made by gc_qsgd_layout", what);
+    GC_REQUIRE(dst->n == n, "%s: the tensors hold %llu elements, the words %llu", what, (unsigned long long)dst->n,
+               (unsigned long long)n);
+    GC_REQUIRE(norm && total_norm && (n == 0 || words), "%s: null pointer", what);
+    GC_REQUIRE(aligned16(words), "%s: words must be 16-byte aligned", what);
+    GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
+    uint64_t at = 0;
+    const uint64_t w0 = reinterpret_cast<uint64_t>(words), m0 = reinterpret_cast<uint64_t>(norm);
+    GC_REQUIRE(!meets(dst, {w0, w0 + 4 * lanes->plane_words}, &at) && !meets(dst, {m0, m0 + 4}, &at),
+               "%s: output tensor %llu shares memory with the words or the norm", what, (unsigned long long)at);
+    hipStream_t st = as_stream(stream);
+    const LaneArg a{words, n, lanes->plane_words, norm, (float)s, alpha, (int32_t)(lanes->world * s), lanes->bits,
+                    lanes->per_word, lanes->world * s};
+    const uint64_t quads = lanes->plane_words >> 2;
+    const unsigned parts =
+        (unsigned)std::min<uint64_t>(std::max<uint64_t>((quads + kNormThreads - 1) / kNormThreads, 1), kNormGrid);
+    uint64_t *part = static_cast<uint64_t *>(workspace);
+    const unsigned grid = scale_grid((lanes->plane_words + 511) / 512);
+    if (p == 2)
+        hipLaunchKernelGGL(k_lane_norm<2>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
+    else if (p == 1)
+        hipLaunchKernelGGL(k_lane_norm<1>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
+    else
+        hipLaunchKernelGGL(k_lane_norm<kPInf>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
+    if (dst->count <= kLdsRecs)
+        hipLaunchKernelGGL((k_decode_clip<true>), dim3(grid), dim3(kScaleThreads), 0, st, a, arg_of(dst), (int)p, max_norm,
+                           part, parts, total_norm);
+    else
+        hipLaunchKernelGGL((k_decode_clip<false>), dim3(grid), dim3(kScaleThreads), 0, st, a, arg_of(dst), (int)p, max_norm,
+                           part, parts, total_norm);
+    return launch_status(what);
+}
+
+}  // extern "C"

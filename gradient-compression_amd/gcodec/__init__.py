@@ -6,6 +6,14 @@ compressors.py / reducer.py / extensions.
 """
 from . import codec  # noqa: F401
 from ._lib import GCodecError  # noqa: F401
+from .clip import (  # noqa: F401
+    Grads,
+    clip_grad_norm_,
+    clip_grads,
+    flatten_clip,
+    grad_norm,
+    qsgd_decode_clip,
+)
 from .compressors import (  # noqa: F401
     GlobalRandKMaxNormCompressor,
     GlobalRandKMaxNormTwoScaleCompressor,

@@ -21,6 +21,9 @@ GC_ENOSPC = -4
 GC_ENODEV = -5
 
 GC_I8, GC_I32, GC_I64 = 1, 4, 8
+GC_F32, GC_F16, GC_BF16 = 16, 17, 18
+GC_NORM_INF = 0
+GC_GRADS_OVERLAP = 1
 GC_RNG_PHILOX, GC_RNG_STREAM, GC_RNG_STREAM24 = 0, 1, 2
 GC_RNG_SPLIT8, GC_RNG_SPLIT16 = 3, 4  # split-plane draws (include/gcodec.h)
 GC_MAX_LEVELS = 8
@@ -78,10 +81,23 @@ class gc_segments(C.Structure):
     ]
 
 
+class gc_grads(C.Structure):
+    _fields_ = [
+        ("count", C.c_uint64),
+        ("n", C.c_uint64),
+        ("rec", C.c_void_p),
+        ("host_rec", C.c_void_p),
+        ("order", C.c_void_p),
+        ("flags", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
 P = C.c_void_p
 u64, u32, i32, f32, i64 = C.c_uint64, C.c_uint32, C.c_int32, C.c_float, C.c_int64
+f64 = C.c_double
 RNGP, LANESP, LEVP = C.POINTER(gc_rng), C.POINTER(gc_lanes), C.POINTER(gc_levels)
-SEGSP = C.POINTER(gc_segments)
+SEGSP, GRADSP = C.POINTER(gc_segments), C.POINTER(gc_grads)
 
 # name -> (restype, argtypes); must match include/gcodec.h exactly
 SIGNATURES = {
@@ -111,6 +127,14 @@ SIGNATURES = {
     "gc_segments_copy": (C.c_int, [SEGSP, SEGSP, f32, P]),
     "gc_qsgd_decode_scatter_segments": (C.c_int, [P, P, u64, P, u32, LANESP, f32, SEGSP, P]),
     "gc_qsgd_decode_segments": (C.c_int, [P, u64, P, u32, LANESP, f32, SEGSP, P]),
+    "gc_grads_plan": (C.c_int, [P, P, P, u64, P, P, GRADSP]),
+    "gc_grads_fill": (C.c_int, [GRADSP, P, P]),
+    "gc_grad_workspace_size": (C.c_size_t, [u64, u64, C.c_int]),
+    "gc_grad_norm": (C.c_int, [GRADSP, u32, P, P, P, P, P]),
+    "gc_grad_norm_root": (C.c_int, [P, u32, P, P]),
+    "gc_grad_clip": (C.c_int, [GRADSP, GRADSP, u32, f64, P, P, P, P]),
+    "gc_grad_flatten_clip": (C.c_int, [GRADSP, P, u32, f64, P, P, P, P]),
+    "gc_qsgd_decode_clip": (C.c_int, [P, u64, P, u32, LANESP, f32, GRADSP, u32, f64, P, P, P]),
     "gc_ms_mask_encode": (C.c_int, [P, P, u64, P, LEVP, RNGP, LANESP, P, P]),
     "gc_ms_select_encode": (C.c_int, [P, P, u64, P, LEVP, RNGP, P, LANESP, LANESP, P, P]),
     "gc_ms_encode_w1": (C.c_int, [P, u64, P, LEVP, RNGP, LANESP, LANESP, P, P, P]),

@@ -42,6 +42,8 @@
  *                              loop reducer.py:543-549 (+ 753-761, 1521-1527, 1705-1711):
  *                              fused flatten + max-norm, decode straight into the per-parameter
  *                              gradients, and the scaled scatter of a flat bucket
+ *   gc_grad_*, gc_qsgd_decode_clip  the global gradient norm and clipping between the
+ *                              reducers and the optimizer step (trainer.py:183-196)
  */
 #ifndef GCODEC_H
 #define GCODEC_H
@@ -301,6 +303,69 @@ int gc_qsgd_decode_scatter_segments(const uint32_t *words, const int64_t *idx, u
 /* gc_qsgd_decode writing each element straight into its tensor (decode + 1/W + setgrad fused) */
 int gc_qsgd_decode_segments(const uint32_t *words, uint64_t n, const float *norm, uint32_t bits,
                             const gc_lanes *lanes, float alpha, const gc_segments *segs, gc_stream_t stream);
+
+/* ---- global gradient norm and clipping ------------------------------------------
+ * A gc_grads describes `count` gradient tensors of GC_F32, GC_F16 or GC_BF16 (mixed
+ * as they come), each contiguous and aligned to its elements, as one sequence of n
+ * elements.  gc_grads_plan builds the host image from (sizes, pointers, types);
+ * gc_grads_fill puts the records on the device, carried in kernel arguments (no
+ * host copy is awaited, so it may be captured).  The caller owns all of it:
+ * rec_host 2 (count + 1) words, order count words, the device copy like rec_host.
+ *
+ *   N = (sum |x|^p)^(1/p) over every element of every tensor, p = 1, 2 or
+ *       GC_NORM_INF (N = max |x|); 0 for no elements; infinities and NaN carry
+ *   c = min(1, max_norm / (N + 1e-6)), NaN where that is NaN
+ *   y = RN_type(RN(x * c)), the product in float32
+ *
+ * Sums are 64-bit floating point in an order fixed by n and the tensor list, so
+ * results repeat bit for bit.  No entry point below uses atomics, keeps state or
+ * needs a zeroed workspace: the workspace (gc_grad_workspace_size bytes, 8-byte
+ * aligned) belongs to the call until its kernels have run.
+ * Replaces, for a list of gradients, what a trainer does between the reducers
+ * (reducer.py:498-554) and the optimizer step (trainer.py:183-196). */
+#define GC_F32 16u
+#define GC_F16 17u
+#define GC_BF16 18u
+#define GC_NORM_INF 0u
+#define GC_GRADS_OVERLAP 1u /* flags: two of the tensors share memory (such a list is only read) */
+typedef struct gc_grads {
+    uint64_t count;           /* tensors */
+    uint64_t n;               /* elements */
+    const uint64_t *rec;      /* device: 2 (count + 1) words, made by gc_grads_fill */
+    const uint64_t *host_rec; /* host: the same words */
+    const uint32_t *order;    /* host: the tensors by address, empty ones last */
+    uint32_t flags;
+    uint32_t reserved;        /* 0 */
+} gc_grads;
+/* host: fills rec_host, order and *out (out->rec is left null) */
+int gc_grads_plan(const uint64_t *sizes, const void *const *ptrs, const uint32_t *types, uint64_t count,
+                  uint64_t *rec_host, uint32_t *order, gc_grads *out);
+int gc_grads_fill(const gc_grads *grads, uint64_t *rec, gc_stream_t stream);
+/* each != 0: with room for the per-tensor norms of gc_grad_norm */
+size_t gc_grad_workspace_size(uint64_t n, uint64_t count, int each);
+/* *norm = N; *total = sum |x|^p (max |x|) in 64 bits, what ranks that hold different
+ * shards add up (take the maximum of); each[count] = the tensors' own norms.  Any of
+ * the three may be NULL */
+int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, float *each, void *workspace,
+                 gc_stream_t stream);
+/* *norm = N of a total */
+int gc_grad_norm_root(const double *total, uint32_t p, float *norm, gc_stream_t stream);
+/* dst = clipped src, tensor by tensor (the same sizes; types may differ), *norm = N (may
+ * be NULL).  total: a device total to clip by (NULL: src's own, computed here).  A
+ * tensor may be clipped onto itself; where that holds for all of them and c = 1,
+ * nothing is written */
+int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double max_norm, const double *total,
+                 float *norm, void *workspace, gc_stream_t stream);
+/* flat[n] = the clipped tensors end to end in float32, *peak = max |flat| (the codec's
+ * max-norm, as gc_segments_flatten_absmax), *norm = N (may be NULL) */
+int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double max_norm, float *peak, float *norm,
+                         void *workspace, gc_stream_t stream);
+/* gc_qsgd_decode's values v = RN(RN(RN(*norm/s) * (lane_sum - W*s)) * alpha), their norm
+ * N = *total_norm, and RN_type(RN(v * c)) into the tensors of dst, which hold n
+ * elements.  The values are never stored unclipped: their norm is taken from the words */
+int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, uint32_t bits, const gc_lanes *lanes,
+                        float alpha, const gc_grads *dst, uint32_t p, double max_norm, float *total_norm,
+                        void *workspace, gc_stream_t stream);
 
 /* ---- multi-scale / two-scale --------------------------------------------- */
 int gc_ms_mask_encode(const float *x, const int64_t *idx, uint64_t n, const float *norm, const gc_levels *levels,

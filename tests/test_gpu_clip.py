@@ -1,0 +1,523 @@
+"""The global gradient norm and clipping (gcodec.clip) on the GPU, against the
+formulas in 64 bits.
+
+Tolerances.  u(t) = eps / 2 is a rounding to type t, relative to the value.
+  norm   a sum of 64-bit terms (each off by 2^-53 at most, the sum of n < 2^33 of
+         them in a tree by less than 64 * 2^-53), then one rounding to float32:
+         2^-24 (1 + 2^-20)
+  clip   c rounds once to float32 (2^-24), the product once (2^-24), the result
+         once to its type: (1 + 2^-24)^2 (1 + u) - 1 < (2^-23 + u)(1 + 2^-6); for
+         a float32 result the product is the result: 2^-23 (1 + 2^-6).  Below the
+         normal range a rounding is off by half the smallest subnormal, absolutely.
+  decode a value rounds 4 times before c: k = RN(norm / s), alpha to float32, RN(k Q),
+         RN(. alpha); a norm of such values is off by as much and rounds once
+         itself (5 times 2^-24), and c takes the norm's 4 (8 more for a result)."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():  # collected on CPU, skipped there
+    pytest.skip("no GPU", allow_module_level=True)
+
+import gcodec  # noqa: E402
+from gcodec import codec, shapes  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+INF = math.inf
+
+RAGGED = [0, 1, 3, 4, 5, 17, 1000, 0, 4099, 70_001, 2, 250_000, 7, 0, 64, 65]
+LISTS = {
+    "one": [1],
+    "only empty": [0, 0],
+    "empty ends": [0, 2047, 0],
+    "a tile": [2048],
+    "past a tile": [2049],
+    "vector ends": [255, 256, 257, 511, 512, 513, 7, 8, 9],
+    "ragged": RAGGED,
+    "one block's": [32_767, 2],
+    "tiny, past the LDS table": [i % 8 for i in range(1500)],
+    "several blocks": [1_000_003, 12, 2_000_001],
+}
+UNIT = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+TINY = {F32: 2.0 ** -149, F16: 2.0 ** -24, BF16: 2.0 ** -133}
+
+
+def types_of(kind, count):
+    return {"fp32": [F32] * count, "fp16": [F16] * count, "bf16": [BF16] * count,
+            "mixed": [(F32, BF16, F16)[i % 3] for i in range(count)]}[kind]
+
+
+def carve(sizes, types, seed, scale=1.0, misalign=True):
+    """Tensors cut from one buffer a type at element offsets of every alignment, with a guard of 7.0 between them."""
+    rng = np.random.default_rng(seed)
+    out = []
+    for s, t in zip(sizes, types):
+        gap = int(rng.integers(1, 16)) if misalign else 16
+        buf = torch.full((gap + s + 16,), 7.0, dtype=t, device=DEV)
+        v = buf[gap:gap + s]
+        v.copy_(torch.from_numpy((rng.standard_normal(s) * scale * 2.0 ** rng.integers(-3, 4)).astype(np.float32)))
+        out.append((buf, gap, v))
+    return out
+
+
+def views(carved):
+    return [v for _, _, v in carved]
+
+
+def guards_hold(carved):
+    for buf, gap, v in carved:
+        assert bool((buf[:gap] == 7).all()) and bool((buf[gap + v.numel():] == 7).all())
+
+
+def f64(ts):
+    return [t.detach().cpu().double().numpy().reshape(-1) for t in ts]
+
+
+def norm64(xs, p):
+    """The formula in 64 bits, exactly rounded sums."""
+    x = np.abs(np.concatenate(xs)) if xs else np.zeros(0)
+    if x.size == 0:
+        return 0.0
+    if p == INF:
+        return float(x.max())
+    if not np.isfinite(x).all():
+        return float("nan") if np.isnan(x).any() else INF
+    return math.fsum(x) if p == 1 else math.sqrt(math.fsum(x * x))
+
+
+def coef64(n, max_norm):
+    q = max_norm / (n + 1e-6)
+    return 1.0 if q > 1.0 else q
+
+
+def close_norm(got, want, roundings=1):
+    got = float(got)
+    if math.isnan(want) or math.isinf(want):
+        assert math.isnan(got) == math.isnan(want) and (math.isnan(want) or got == want)
+    else:
+        assert abs(got - want) <= roundings * 2.0 ** -24 * (1 + 2.0 ** -6) * want, (got, want)
+
+
+def close_values(got, want, extra=0):
+    """got tensors of their types against 64-bit values; `extra` more float32 roundings"""
+    for g, w in zip(got, want):
+        u = UNIT[g.dtype]
+        rel = ((2 + extra) * 2.0 ** -24 + (u if g.dtype != F32 else 0.0)) * (1 + 2.0 ** -6)
+        tol = rel * np.abs(w) + TINY[g.dtype] * 0.5 + (1 + extra) * 2.0 ** -150
+        err = np.abs(g.detach().cpu().double().numpy().reshape(-1) - w)
+        assert (err <= tol).all(), (g.dtype, g.shape, float((err - tol).max()))
+
+
+# ---------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16", "mixed"])
+@pytest.mark.parametrize("name", list(LISTS))
+def test_norm(name, kind, p):
+    sizes = LISTS[name]
+    ts = views(carve(sizes, types_of(kind, len(sizes)), seed=len(sizes)))
+    xs = f64(ts)
+    close_norm(gcodec.grad_norm(ts, p), norm64(xs, p))
+    total, each = gcodec.grad_norm(gcodec.Grads(ts), p, per_tensor=True)
+    close_norm(total, norm64(xs, p))
+    assert each.shape == (len(sizes),) and each.dtype == F32
+    for e, x in zip(each.tolist(), xs):
+        close_norm(e, norm64([x], p))
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("scale", [1e-30, 1e-42, 1e30])
+def test_norm_of_extreme_gradients(scale, p):
+    """Squares that float32 cannot hold, and subnormal elements."""
+    ts = views(carve([5000, 33, 1], [F32] * 3, seed=3, scale=scale))
+    want = norm64(f64(ts), p)
+    got = float(gcodec.grad_norm(ts, p))
+    assert abs(got - want) <= 2.0 ** -24 * (1 + 2.0 ** -6) * want + 2.0 ** -150
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("bad", [INF, -INF, math.nan])
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
+def test_norm_carries_infinities_and_nan(kind, bad, p):
+    ts = views(carve([3000, 70, 9], types_of(kind, 3), seed=5))
+    ts[1][69] = bad
+    total, each = gcodec.grad_norm(ts, p, per_tensor=True)
+    want = math.nan if math.isnan(bad) else INF
+    close_norm(total, want)
+    close_norm(each[1], want)
+    assert math.isfinite(each[0]) and math.isfinite(each[2])
+    ts[0][0] = math.nan  # a NaN is above an infinity
+    close_norm(gcodec.grad_norm(ts, p), math.nan)
+    with pytest.raises(RuntimeError, match="not finite"):
+        gcodec.grad_norm(ts, p, error_if_nonfinite=True)
+
+
+def test_norm_repeats_bit_for_bit():
+    ts = views(carve([3_000_001, 5, 40_000], [F32, BF16, F16], seed=8))
+    g = gcodec.Grads(ts)
+    first = gcodec.grad_norm(g, 2, per_tensor=True)
+    for _ in range(5):
+        again = gcodec.grad_norm(ts, 2, per_tensor=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_norm_past_32_bit_offsets():
+    """2^32 + 70,001 elements, two tensors: the far end counts and is clipped, the rest stays."""
+    n = 2 ** 32 + 65_536
+    a, b = torch.zeros(n, dtype=BF16, device=DEV), torch.zeros(4465, dtype=BF16, device=DEV)
+    a[-1], a[2 ** 32 + 1], a[3], b[-1] = 3.0, 4.0, 12.0, 84.0
+    assert float(gcodec.grad_norm([a, b], 2)) == 85.0  # sqrt(9 + 16 + 144 + 7056)
+    assert float(gcodec.grad_norm([a, b], INF)) == 84.0
+    total, each = gcodec.grad_norm([a, b], 1, per_tensor=True)
+    assert float(total) == 103.0 and each.tolist() == [19.0, 84.0]
+    w, v = torch.nn.Parameter(a), torch.nn.Parameter(b)  # the gradient is the parameter itself: in place
+    w.grad, v.grad = w.data, v.data
+    gcodec.clip_grad_norm_([w, v], 42.5)
+    assert [float(x) for x in (a[-1], a[2 ** 32 + 1], a[3], b[-1])] == [1.5, 2.0, 6.0, 42.0]
+    assert int(torch.count_nonzero(a)) == 3 and int(torch.count_nonzero(b)) == 1
+
+
+# ---------------------------------------------------------------------------
+# clip
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("factor", [0.37, 3.0])
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16", "mixed"])
+@pytest.mark.parametrize("name", list(LISTS))
+def test_clip_list_to_list(name, kind, p, factor):
+    sizes = LISTS[name]
+    types = types_of(kind, len(sizes))
+    src, dst = carve(sizes, types, seed=11), carve(sizes, types[1:] + types[:1], seed=12)
+    xs = f64(views(src))
+    n = norm64(xs, p)
+    m = factor * n if n else 1.0
+    total = gcodec.clip_grads(views(src), views(dst), m, p)
+    close_norm(total, n)
+    close_values(views(dst), [x * coef64(n, m) for x in xs])
+    guards_hold(dst)
+    for x, t in zip(xs, views(src)):
+        assert np.array_equal(x, t.cpu().double().numpy())  # read only
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16", "mixed"])
+@pytest.mark.parametrize("name", ["one", "ragged", "tiny, past the LDS table", "several blocks"])
+def test_clip_in_place(name, kind, p):
+    sizes = LISTS[name]
+    grads = carve(sizes, types_of(kind, len(sizes)), seed=21)
+    params = [torch.nn.Parameter(torch.zeros_like(g)) for g in views(grads)]
+    params.insert(1, torch.nn.Parameter(torch.zeros(3, device=DEV)))  # without a gradient
+    for q, g in zip(params[:1] + params[2:], views(grads)):
+        q.grad = g
+    xs = f64(views(grads))
+    n = norm64(xs, p)
+    before = [g.clone() for g in views(grads)]
+    version = views(grads)[0]._version
+    close_norm(gcodec.clip_grad_norm_(params, 2 * n + 1, p), n)  # under the limit: nothing changes
+    for a, b in zip(before, views(grads)):
+        assert torch.equal(a, b)
+    close_norm(gcodec.clip_grad_norm_(iter(params), 0.4 * n, p), n)
+    close_values(views(grads), [x * coef64(n, 0.4 * n) for x in xs])
+    guards_hold(grads)
+    assert views(grads)[0]._version > version  # autograd sees the write
+
+
+def test_clip_agrees_with_the_trainer_call():
+    """torch.nn.utils.clip_grad_norm_ on float32: its norm is a float32 sum, here within 2^-16 of ours."""
+    grads = views(carve(shapes.vgg16_sizes()[:20], [F32] * 20, seed=31, scale=1e-2))
+    mine = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+    ref = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+    for a, b, g in zip(mine, ref, grads):
+        a.grad, b.grad = g.clone(), g.clone()
+    na, nb = gcodec.clip_grad_norm_(mine, 1.0), torch.nn.utils.clip_grad_norm_(ref, 1.0)
+    assert na.shape == nb.shape and na.dtype == nb.dtype
+    torch.testing.assert_close(na, nb, rtol=2.0 ** -16, atol=0)
+    for a, b in zip(mine, ref):
+        torch.testing.assert_close(a.grad, b.grad, rtol=2.0 ** -15, atol=0)
+
+
+@pytest.mark.parametrize("max_norm", [0.0, INF, 1.0])
+@pytest.mark.parametrize("bad", [None, INF, -INF, math.nan])
+def test_clip_limits_and_nonfinite_gradients(bad, max_norm):
+    """max_norm 0 clears, infinity leaves; an infinite norm gives c = 0 (NaN where the gradient is infinite, 0
+    elsewhere), a NaN or infinity over infinity NaN everywhere: the formula's own values."""
+    ts = views(carve([300, 5000], [F32, BF16], seed=41))
+    if bad is not None:
+        ts[0][7] = bad
+    xs = f64(ts)
+    n = norm64(xs, 2)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        c = np.float64(max_norm) / (np.float64(n) + 1e-6)
+        c = 1.0 if c > 1.0 else c
+        want = [x * c for x in xs]
+    outs = [torch.full_like(t, 5.0) for t in ts]
+    close_norm(gcodec.clip_grads(ts, outs, max_norm), n)
+    for o, w in zip(outs, want):
+        g = o.cpu().double().numpy()
+        assert np.array_equal(np.isnan(g), np.isnan(w))
+        ok = ~np.isnan(w)
+        assert (np.abs(g[ok] - w[ok]) <= (2.0 ** -23 + UNIT[o.dtype]) * 1.02 * np.abs(w[ok])).all()
+    if bad is not None:
+        params = [torch.nn.Parameter(torch.zeros_like(t)) for t in ts]
+        for q, t in zip(params, ts):
+            q.grad = t
+        with pytest.raises(RuntimeError, match="not finite"):
+            gcodec.clip_grad_norm_(params, max_norm, error_if_nonfinite=True)
+        for x, t in zip(xs, ts):
+            assert np.array_equal(x, t.cpu().double().numpy(), equal_nan=True)  # raised before anything was written
+
+
+def test_clip_partly_in_place_and_dense_orders():
+    a, b = views(carve([1000, 300], [F32, BF16], seed=51))
+    out = torch.zeros(300, device=DEV)
+    xs = f64([a, b])
+    n = norm64(xs, 2)
+    gcodec.clip_grads([a, b], [a, out], 0.5 * n)  # the first onto itself, the second elsewhere
+    close_values([a, out], [x * coef64(n, 0.5 * n) for x in xs])
+    w = torch.nn.Parameter(torch.randn(8, 6, 5, 4, device=DEV).to(memory_format=torch.channels_last))
+    w.grad = torch.randn(8, 6, 5, 4, device=DEV).to(memory_format=torch.channels_last)
+    assert not w.grad.is_contiguous()
+    x = w.grad.cpu().double().numpy()
+    n = norm64([x.reshape(-1)], 2)
+    close_norm(gcodec.grad_norm([w.grad]), n)
+    gcodec.clip_grad_norm_(w, 0.5 * n)  # one parameter, not a list
+    close_values([w.grad.contiguous()], [(x * coef64(n, 0.5 * n)).reshape(-1)])
+
+
+def test_refusals():
+    x = torch.ones(8, 8, device=DEV)
+    y = torch.ones(64, device=DEV)
+    E = gcodec.GCodecError
+    for bad in ([x[:, :4]], [x.t()], [x.double()], [x.to(torch.int32)], [x.cpu()], [x, x.cpu()], [x.to_sparse()], []):
+        with pytest.raises(E):
+            gcodec.Grads(bad)
+    with pytest.raises(E, match="not dense"):
+        gcodec.grad_norm([x[:, :4]])
+    with pytest.raises(E, match="not dense"):
+        gcodec.grad_norm([y[:1].expand(4)])
+    with pytest.raises(E, match="share memory"):
+        gcodec.clip_grads([y, y], [y, y], 1.0)
+    with pytest.raises(E, match="shares memory"):
+        gcodec.clip_grads([y[:32]], [y[16:48]], 1.0)
+    with pytest.raises(E, match="sizes"):
+        gcodec.clip_grads([x, y], [y[:63], torch.empty(65, device=DEV)], 1.0)
+    with pytest.raises(E, match="tensors into"):
+        gcodec.clip_grads([x, y], [torch.empty_like(y)], 1.0)
+    with pytest.raises(E, match="flat"):
+        gcodec.flatten_clip([y], 1.0, flat=torch.empty(63, device=DEV))
+    with pytest.raises(E, match="float32"):
+        gcodec.flatten_clip([y], 1.0, flat=torch.empty(64, device=DEV, dtype=F16))
+    with pytest.raises(E, match="flat bucket"):
+        gcodec.flatten_clip([y], 1.0, flat=y)
+    words = torch.zeros(codec.qsgd_layout(64, 4).plane_words, dtype=torch.int32, device=DEV)
+    one = torch.ones(1, device=DEV)
+    for w, kw, msg in [(words[:4], {}, "needed"), (words.float(), {}, "int32"), (words.cpu(), {}, "GPU only"),
+                       (words, dict(lanes=codec.qsgd_layout(63, 4)), "n=63"), (words, dict(lanes=codec.qsgd_layout(64, 2)), "lanes")]:
+        with pytest.raises(E, match=msg):
+            gcodec.qsgd_decode_clip(w, one, 4, [torch.empty(64, device=DEV)], 1.0, **kw)
+    with pytest.raises(E, match="empty norm"):
+        gcodec.qsgd_decode_clip(words, one[:0], 4, [torch.empty(64, device=DEV)], 1.0)
+
+
+# ---------------------------------------------------------------------------
+# flatten
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("factor", [0.37, 3.0])
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "mixed"])
+@pytest.mark.parametrize("name", list(LISTS))
+def test_flatten(name, kind, p, factor):
+    sizes = LISTS[name]
+    ts = views(carve(sizes, types_of(kind, len(sizes)), seed=61))
+    xs = f64(ts)
+    n = norm64(xs, p)
+    m = factor * n if n else 1.0
+    store = torch.full((sum(sizes) + 9,), 7.0, device=DEV)
+    out = store[5:5 + sum(sizes)]
+    flat, peak, total = gcodec.flatten_clip(ts, m, p, flat=out)
+    assert flat.data_ptr() == out.data_ptr() and peak.shape == (1,)
+    close_norm(total, n)
+    close_values([flat], [np.concatenate(xs) * coef64(n, m)])
+    assert bool((store[:5] == 7).all()) and bool((store[5 + sum(sizes):] == 7).all())
+    assert float(peak) == (float(flat.abs().max()) if flat.numel() else 0.0)  # the codec's max-norm, exactly
+
+
+@pytest.mark.parametrize("bad", [INF, math.nan])
+def test_flatten_nonfinite(bad):
+    ts = views(carve([100, 3000], [F32, BF16], seed=62))
+    ts[1][8] = bad
+    flat, peak, total = gcodec.flatten_clip(ts, 1.0)
+    assert math.isnan(float(peak)) and math.isnan(float(flat.abs().max()))
+    close_norm(total, bad)
+
+
+# ---------------------------------------------------------------------------
+# decode
+# ---------------------------------------------------------------------------
+def packed(n, bits, world, seed, norm=0.02):
+    """Words of random levels summed over `world` ranks, by the codec's own packer."""
+    rng = np.random.default_rng(seed)
+    s = (1 << bits) - 1
+    q = np.zeros(n, dtype=np.int64)
+    for _ in range(world):
+        q += np.clip(np.rint(rng.standard_normal(n) * s / 4), -s, s).astype(np.int64)
+    if n:
+        q[0] = world * s
+    lanes = codec.qsgd_layout(n, bits, world)
+    words = torch.zeros(lanes.plane_words, dtype=torch.int64, device=DEV)
+    lane = torch.from_numpy(q + world * s).to(DEV)
+    for k in range(lanes.per_word):
+        part = lane[k * lanes.plane_words:(k + 1) * lanes.plane_words]
+        words[:part.numel()] += part << (k * lanes.bits)
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+    return words, q, torch.tensor([norm], dtype=F32, device=DEV)
+
+
+@pytest.mark.parametrize("factor", [0.37, 3.0])
+@pytest.mark.parametrize("bits,world,p", [(1, 1, 2), (2, 1, 1), (4, 1, 2), (4, 1, INF), (4, 3, 2), (8, 8, 2), (8, 1, 1),
+                                          (12, 2, 2), (16, 8, 2), (20, 1, 1), (24, 1, INF)])
+@pytest.mark.parametrize("name,kind", [("one", "fp32"), ("empty ends", "bf16"), ("ragged", "mixed"), ("ragged", "fp32"),
+                                       ("tiny, past the LDS table", "fp16"), ("several blocks", "bf16")])
+def test_decode(name, kind, bits, world, p, factor):
+    sizes = LISTS[name]
+    n = sum(sizes)
+    words, q, norm = packed(n, bits, world, seed=bits)
+    dst = carve(sizes, types_of(kind, len(sizes)), seed=71)
+    flat = q * (float(norm) / ((1 << bits) - 1) / world)
+    parts = np.split(flat, np.cumsum(sizes)[:-1])
+    want = norm64([flat], p)
+    m = factor * want
+    total = gcodec.qsgd_decode_clip(words, norm, bits, views(dst), m, p, world=world, alpha=1.0 / world)
+    close_norm(total, want, roundings=5)
+    close_values(views(dst), [x * coef64(want, m) for x in parts], extra=8)
+    guards_hold(dst)
+
+
+@pytest.mark.parametrize("bits,world", [(2, 1), (4, 3), (8, 8), (16, 1)])
+def test_decode_unclipped_is_the_decode(bits, world):
+    """Under the limit the values are qsgd_decode_segments' own, bit for bit."""
+    ts = views(carve(RAGGED, [F32] * len(RAGGED), seed=81))
+    us = views(carve(RAGGED, [F32] * len(RAGGED), seed=82))
+    words, _, norm = packed(sum(RAGGED), bits, world, seed=9)
+    codec.qsgd_decode_segments(words, norm, bits, codec.Segments(ts), world, 1.0 / world)
+    gcodec.qsgd_decode_clip(words, norm, bits, us, INF, world=world, alpha=1.0 / world)
+    for a, b in zip(ts, us):
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("norm", [0.0, 1e-44, 1e-20, 3e38, INF, math.nan])
+def test_decode_extreme_norms(norm, p):
+    """The norm is that of the decoded values also where they leave the normal range or are not finite."""
+    words, q, nt = packed(5000, 4, 2, seed=3, norm=norm)
+    plain = [torch.empty(5000, device=DEV)]
+    codec.qsgd_decode_segments(words, nt, 4, codec.Segments(plain), 2, 1.0)  # alpha 1: W max-norms may pass float32
+    xs = f64(plain)
+    want = norm64(xs, p)
+    out = [torch.empty(5000, device=DEV)]
+    total = gcodec.qsgd_decode_clip(words, nt, 4, out, 1.0, p, world=2, alpha=1.0)
+    if want > 3.4028235e38:
+        want = INF
+    if math.isfinite(want):
+        assert abs(float(total) - want) <= 2.0 ** -22 * want + 2.0 ** -150
+    else:
+        close_norm(total, want)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        w64 = norm64(xs, p)
+        w = xs[0] * coef64(w64, 1.0)
+    g = out[0].cpu().double().numpy()
+    assert np.array_equal(np.isnan(g), np.isnan(w))
+    ok = ~np.isnan(w)
+    assert (np.abs(g[ok] - w[ok]) <= 2.0 ** -22 * np.abs(w[ok]) + 2.0 ** -149).all()
+
+
+# ---------------------------------------------------------------------------
+# together, streams, graphs
+# ---------------------------------------------------------------------------
+def test_a_step_with_all_of_them():
+    """Local clipping into the codec, and the reduced gradient clipped as it is decoded (one rank)."""
+    sizes = [27, 64, 0, 1000, 3, 4099, 10, 70_001]
+    ts = views(carve(sizes, types_of("mixed", len(sizes)), seed=91, scale=0.01))
+    outs = carve(sizes, types_of("mixed", len(sizes)), seed=92)
+    xs = f64(ts)
+    flat, peak, total = gcodec.flatten_clip(ts, 0.5)
+    close_norm(total, norm64(xs, 2))
+    words = codec.qsgd_encode(flat, peak, 8, gcodec.Generator(5, "philox").reserve(flat.numel()))
+    dense = codec.qsgd_decode(words, flat.numel(), peak, 8)
+    n = gcodec.qsgd_decode_clip(words, peak, 8, views(outs), 0.3)
+    want = dense.cpu().double().numpy()
+    close_norm(n, norm64([want], 2), roundings=4)
+    c = coef64(norm64([want], 2), 0.3)
+    close_values(views(outs), [x * c for x in np.split(want, np.cumsum(sizes)[:-1])], extra=1)
+    after = gcodec.grad_norm(views(outs))
+    assert abs(float(after) - 0.3) < 0.3 * 2.0 ** -7  # what was stored has the limit's norm, to bf16's rounding
+
+
+def test_two_streams_at_once():
+    a = views(carve([2_000_001, 17], [F32, BF16], seed=101))
+    b = views(carve([1_500_000, 999], [BF16, F32], seed=102))
+    ga, gb = gcodec.Grads(a), gcodec.Grads(b)
+    wa, wb = gcodec.grad_norm(ga), gcodec.grad_norm(gb)
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(sa):
+            got.append((gcodec.grad_norm(ga), wa))
+        with torch.cuda.stream(sb):
+            got.append((gcodec.grad_norm(gb), wb))
+            got.append((gcodec.grad_norm(ga), wa))  # one table on two streams
+    torch.cuda.synchronize()
+    for x, w in got:
+        assert torch.equal(x, w)
+
+
+def test_captured_and_replayed():
+    """Two graphs, lists and tables, replayed between eager calls with new gradients each time."""
+    src, dst = carve(RAGGED, types_of("mixed", len(RAGGED)), seed=111), carve(RAGGED, [F32] * len(RAGGED), seed=112)
+    s, d = views(src), views(dst)
+    gs, gd = gcodec.Grads(s), gcodec.Grads(d)
+    gcodec.clip_grads(gs, gd, 1.0)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        n1 = gcodec.clip_grads(gs, gd, 1.0)
+        with pytest.raises(gcodec.GCodecError, match="capture"):
+            gcodec.Grads(s)
+    with torch.cuda.graph(two):
+        flat, peak, n2 = gcodec.flatten_clip(s, 2.0)
+        n3, each = gcodec.grad_norm(s, 1, per_tensor=True)
+    for step in range(4):
+        with torch.no_grad():
+            for t in s:
+                t.mul_(-1.5)
+        xs = f64(s)
+        two.replay()
+        one.replay()
+        close_norm(gcodec.grad_norm(s, INF), norm64(xs, INF))  # eager work between the replays
+        torch.cuda.synchronize()
+        n = norm64(xs, 2)
+        close_norm(n1, n)
+        close_norm(n2, n)
+        close_norm(n3, norm64(xs, 1))
+        close_values(d, [x * coef64(n, 1.0) for x in xs])
+        close_values([flat], [np.concatenate(xs) * coef64(n, 2.0)])
+        assert float(peak) == float(flat.abs().max())
+        for e, x in zip(each.tolist(), xs):
+            close_norm(e, norm64([x], 1))
+
+
+def test_table_keeps_its_memory():
+    """A table made of tensors that are dropped still reads their memory, not a later tensor's."""
+    t = torch.full((1 << 20,), 2.0, device=DEV)
+    g = gcodec.Grads([t])
+    del t
+    other = [torch.full((1 << 20,), 9.0, device=DEV) for _ in range(4)]
+    assert float(gcodec.grad_norm(g, INF)) == 2.0
+    del other
