@@ -10,7 +10,8 @@
 // partials in one fixed order and forms c itself.  So there are no atomics, no
 // tickets and no zeroed state: the result does not depend on the schedule, a
 // captured call owns all that it writes, and two calls on different streams
-// share nothing.
+// share nothing.  What one block can read in a few microseconds (kOneTiles) is
+// done by one block in one launch.
 //
 // Sums are held in 64 bits: the square of a float32 is exact to half an ulp
 // there and cannot overflow or vanish, so N is right for any gradients whose
@@ -28,7 +29,7 @@
 #include <math.h>
 
 #include <algorithm>
-#include <vector>
+#include <type_traits>
 
 namespace gc {
 
@@ -37,6 +38,7 @@ constexpr unsigned kNormThreads = 1024;
 constexpr unsigned kNormGrid = 512;    // two blocks a CU: 32 waves, each with 4 KB in flight
 constexpr unsigned kScaleThreads = 256;
 constexpr unsigned kScaleGrid = 2048;
+constexpr uint64_t kOneTiles = 16;     // a tile a wave of one block
 constexpr double kEps = 1e-6;
 
 // workspace: kNormGrid partials (64-bit), kNormGrid maxima (32-bit), then the
@@ -136,28 +138,20 @@ __device__ __forceinline__ void wave_read_any(uint32_t type, uint64_t base, uint
         wave_read<_Float16>(glob<const _Float16>(base, off), cnt, f);
 }
 
-// One partial of |x|^p a block (and, PEAK, one of max |x|).  EACH: also the sum
-// of every piece, at slot (tile + tensor): along the flat sequence each next
-// piece has the next tile or the next tensor, so a tensor's pieces have
-// consecutive slots of their own.
-template <int P, bool EACH, bool PEAK, bool LDS>
-__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, double *__restrict__ part,
-                                                            uint32_t *__restrict__ peak, double *__restrict__ slots)
+// The block's share of the sum of |x|^p and (PEAK) of max |x|, valid in thread 0.
+// EACH: also the sum of every piece, at slot (tile + tensor): along the flat
+// sequence each next piece has the next tile or the next tensor, so a tensor's
+// pieces have consecutive slots of their own.
+template <int P, bool EACH, bool PEAK>
+__device__ __forceinline__ void block_norm(const GradRec *rec, uint32_t count, uint64_t n, double *__restrict__ slots,
+                                           Acc<P> &all, Acc<kPInf> &top)
 {
-    __shared__ GradRec srec[LDS ? kLdsRecs + 1 : 1];
     __shared__ double sacc[kNormThreads / 64];
     __shared__ uint32_t smax[kNormThreads / 64];
-    const GradRec *rec = LDS ? srec : g.rec;
-    if (LDS && n) {
-        stage_table(g, srec);
-        __syncthreads();
-    }
-    Acc<P> all;
-    Acc<kPInf> top;
     const uint64_t tiles = (n + kTile - 1) / kTile, waves = (uint64_t)gridDim.x * (kNormThreads / 64);
     for (uint64_t t = (uint64_t)blockIdx.x * (kNormThreads / 64) + wave_id(); t < tiles; t += waves) {
         const uint64_t lo = t * kTile, hi = min(lo + kTile, n);
-        grad_walk(rec, g.count, lo, hi,
+        grad_walk(rec, count, lo, hi,
                   [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
                       Acc<P> one;
                       Acc<P> &acc = EACH ? one : all;
@@ -183,7 +177,7 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
             smax[wave_id()] = top.m;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0)
         for (unsigned w = 1; w < kNormThreads / 64; ++w) {
             Acc<P> o;
             o.set(sacc[w]);
@@ -191,10 +185,6 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
             if (PEAK)
                 top.m = max(top.m, smax[w]);
         }
-        part[blockIdx.x] = all.value();
-        if (PEAK)
-            peak[blockIdx.x] = top.m;
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -203,8 +193,22 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
 template <int P>
 __device__ __forceinline__ double wave_total(const double *__restrict__ part, uint32_t parts)
 {
+    constexpr uint32_t U = 8;  // loads in flight: a large tensor has tens of thousands of slots
     Acc<P> a;
-    for (uint32_t i = lane_id(); i < parts; i += 64) {
+    uint32_t i = lane_id();
+    for (; i + (U - 1) * 64 < parts; i += U * 64) {
+        double v[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            v[u] = part[i + u * 64];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            Acc<P> o;
+            o.set(v[u]);
+            a.join(o);
+        }
+    }
+    for (; i < parts; i += 64) {
         Acc<P> o;
         o.set(part[i]);
         a.join(o);
@@ -227,44 +231,80 @@ __device__ __forceinline__ float clip_coef(double norm, double max_norm)
     return q > 1.0 ? 1.0f : (float)q;
 }
 
-// block 0: the total and N; block 1 + s (EACH): the norm of tensor s
-__global__ __launch_bounds__(kScaleThreads) void k_grad_finish(GradArg g, int p, const double *__restrict__ part,
-                                                               uint32_t parts, const double *__restrict__ slots,
+__device__ __forceinline__ void write_norm(int p, double t, double *total, float *norm)
+{
+    if (total)
+        *total = t;
+    if (norm)
+        *norm = (float)root_of(p, t);
+}
+
+// the norm of tensor s from its slots; the wave's, or (WAVES > 1) the block's:
+// the same number of slots for every wave's share, then the waves in order
+template <int P, unsigned WAVES>
+__device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, const double *slots, float *__restrict__ each)
+{
+    const uint64_t a = uni64(rec[s].start), b = uni64(rec[s + 1].start);
+    double t = 0.0;
+    if (a != b) {
+        const uint64_t s0 = a / kTile + s, cnt = (b - 1) / kTile + s + 1 - s0;
+        const uint64_t share = (cnt + WAVES - 1) / WAVES, w0 = WAVES > 1 ? wave_id() * share : 0;
+        t = wave_total<P>(slots + s0 + w0, w0 < cnt ? (uint32_t)min(share, cnt - w0) : 0u);
+    }
+    if constexpr (WAVES > 1) {
+        __shared__ double sw[WAVES];
+        if (lane_id() == 0)
+            sw[wave_id()] = t;
+        __syncthreads();
+        if (wave_id() != 0)
+            return;
+        t = wave_total<P>(sw, WAVES);
+    }
+    if (lane_id() == 0)
+        each[s] = (float)root_of(P, t);
+}
+
+// One partial a block; a grid of one block finishes the call itself
+template <int P, bool EACH, bool PEAK, bool LDS>
+__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, double *__restrict__ part,
+                                                               uint32_t *__restrict__ peak, double *slots,
                                                                double *__restrict__ total, float *__restrict__ norm,
                                                                float *__restrict__ each)
 {
-    if (blockIdx.x == 0) {
-        if (wave_id() == 0) {
-            const double t = wave_total_of(p, part, parts);
-            if (lane_id() == 0) {
-                if (total)
-                    *total = t;
-                if (norm)
-                    *norm = (float)root_of(p, t);
-            }
-        }
-        return;
+    __shared__ GradRec srec[LDS ? kLdsRecs + 1 : 1];
+    const GradRec *rec = LDS ? srec : g.rec;
+    if (LDS && g.count) {
+        stage_table(g, srec);
+        __syncthreads();
     }
-    __shared__ double sw[kScaleThreads / 64];
-    const uint32_t s = blockIdx.x - 1;
-    const uint64_t a = g.rec[s].start, b = g.rec[s + 1].start;
-    if (a == b) {
-        if (threadIdx.x == 0)
-            each[s] = 0.0f;
-        return;
+    Acc<P> all;
+    Acc<kPInf> top;
+    block_norm<P, EACH, PEAK>(rec, g.count, n, slots, all, top);
+    if (threadIdx.x == 0) {
+        part[blockIdx.x] = all.value();
+        if (PEAK)
+            peak[blockIdx.x] = top.m;
+        if (gridDim.x == 1)
+            write_norm(P, all.value(), total, norm);
     }
-    // the same number of slots for every wave's share, then the waves in order
-    const uint64_t s0 = a / kTile + s, cnt = (b - 1) / kTile + s + 1 - s0;
-    const uint64_t share = (cnt + kScaleThreads / 64 - 1) / (kScaleThreads / 64), w0 = wave_id() * share;
-    const uint64_t mine = w0 < cnt ? min(share, cnt - w0) : 0;
-    const double t = wave_total_of(p, slots + s0 + w0, (uint32_t)mine);
-    if (lane_id() == 0)
-        sw[wave_id()] = t;
-    __syncthreads();
-    if (wave_id() == 0) {
-        const double r = wave_total_of(p, sw, kScaleThreads / 64);
+    if (EACH && gridDim.x == 1)  // behind block_norm's barrier, which the slots' writes are ahead of
+        for (uint32_t s = wave_id(); s < g.count; s += kNormThreads / 64)
+            tensor_norm<P, 1>(rec, s, slots, each);
+}
+
+// block 0: the total and N; block 1 + s: the norm of tensor s
+template <int P>
+__global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, const double *__restrict__ part, uint32_t parts,
+                                                              const double *__restrict__ slots,
+                                                              double *__restrict__ total, float *__restrict__ norm,
+                                                              float *__restrict__ each)
+{
+    if (blockIdx.x > 0) {
+        tensor_norm<P, kNormThreads / 64>(g.rec, blockIdx.x - 1, slots, each);
+    } else if (wave_id() == 0) {
+        const double t = wave_total<P>(part, parts);
         if (lane_id() == 0)
-            each[s] = (float)root_of(p, r);
+            write_norm(P, t, total, norm);
     }
 }
 
@@ -319,9 +359,29 @@ __device__ __forceinline__ void wave_scale_to(uint32_t td, Glob<const TS> x, uin
         wave_scale<TS, _Float16>(x, glob<_Float16>(base, off), cnt, c);
 }
 
-// y = RN(x c) from the tensors of src into those of dst (the same sizes), or
-// (FLAT) end to end into float32.  The partials' pass has c = 1 in most steps
-// of a training run; in place nothing is left to do then.
+// Tile t of y = RN(x c), from the tensors of src into those of dst (the same
+// sizes), or (FLAT) end to end into float32
+template <bool FLAT>
+__device__ __forceinline__ void scale_tile(const GradRec *rs, const GradRec *rd, uint32_t count, float *flat, uint64_t n,
+                                           uint64_t t, float c)
+{
+    const uint64_t lo = t * kTile, hi = min(lo + kTile, n);
+    grad_walk(rs, count, lo, hi, [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
+        const uint64_t dpt = FLAT ? (uint64_t)kTF32 << 56 | reinterpret_cast<uint64_t>(flat) : uni64(rd[s].pt);
+        const uint64_t off = a - start, doff = FLAT ? a : off;
+        const uint32_t td = (uint32_t)(dpt >> 56), cnt = (uint32_t)(b - a);
+        const uint64_t dbase = dpt & 0x00ffffffffffffffull;
+        if (type == kTF32)
+            wave_scale_to<float>(td, glob<const float>(base, off), dbase, doff, cnt, c);
+        else if (type == kTBF16)
+            wave_scale_to<__bf16>(td, glob<const __bf16>(base, off), dbase, doff, cnt, c);
+        else
+            wave_scale_to<_Float16>(td, glob<const _Float16>(base, off), dbase, doff, cnt, c);
+    });
+}
+
+// The partials' pass has c = 1 in most steps of a training run; in place
+// nothing is left to do then.
 template <bool FLAT, bool LDS>
 __global__ __launch_bounds__(kScaleThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n, int p,
                                                               double max_norm, const double *__restrict__ part,
@@ -357,22 +417,43 @@ __global__ __launch_bounds__(kScaleThreads) void k_grad_scale(GradArg src, GradA
         __syncthreads();
     }
     const uint64_t tiles = (n + kTile - 1) / kTile, waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
-    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves) {
-        const uint64_t lo = (tiles - 1 - t) * kTile, hi = min(lo + kTile, n);
-        grad_walk(rs, src.count, lo, hi,
-                  [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
-                      const uint64_t dpt = FLAT ? (uint64_t)kTF32 << 56 | reinterpret_cast<uint64_t>(flat) : uni64(rd[s].pt);
-                      const uint64_t off = a - start, doff = FLAT ? a : off;
-                      const uint32_t td = (uint32_t)(dpt >> 56), cnt = (uint32_t)(b - a);
-                      const uint64_t dbase = dpt & 0x00ffffffffffffffull;
-                      if (type == kTF32)
-                          wave_scale_to<float>(td, glob<const float>(base, off), dbase, doff, cnt, c);
-                      else if (type == kTBF16)
-                          wave_scale_to<__bf16>(td, glob<const __bf16>(base, off), dbase, doff, cnt, c);
-                      else
-                          wave_scale_to<_Float16>(td, glob<const _Float16>(base, off), dbase, doff, cnt, c);
-                  });
+    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves)
+        scale_tile<FLAT>(rs, rd, src.count, flat, n, tiles - 1 - t, c);
+}
+
+// both passes in one block
+template <int P, bool FLAT>
+__global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, GradArg dst, float *flat, uint64_t n,
+                                                                double max_norm, bool in_place, float *__restrict__ norm,
+                                                                float *__restrict__ peak)
+{
+    __shared__ GradRec ss[kLdsRecs + 1];
+    __shared__ GradRec sd[FLAT ? 1 : kLdsRecs + 1];
+    __shared__ float sc;
+    if (n) {
+        stage_table(src, ss);
+        if (!FLAT)
+            stage_table(dst, sd);
+        __syncthreads();
     }
+    Acc<P> all;
+    Acc<kPInf> top;
+    block_norm<P, false, FLAT>(ss, src.count, n, nullptr, all, top);
+    if (threadIdx.x == 0) {
+        const double N = root_of(P, all.value());
+        sc = clip_coef(N, max_norm);
+        if (norm)
+            *norm = (float)N;
+        if (FLAT)
+            *peak = __uint_as_float(top.m) * sc;
+    }
+    __syncthreads();
+    const float c = sc;
+    if (in_place && c == 1.0f)
+        return;
+    const uint64_t tiles = (n + kTile - 1) / kTile;
+    for (uint64_t t = wave_id(); t < tiles; t += kNormThreads / 64)
+        scale_tile<FLAT>(ss, sd, src.count, flat, n, t, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -401,81 +482,123 @@ __device__ __forceinline__ bool lanes_exact(const LaneArg &a, float k)
     return a.w <= 14 && step >= 1e-30 && step <= 1e30 && top <= 1e38 && top * fabs((double)a.alpha) <= 1e38;
 }
 
+// A partial is the exact integer sum, or the bits of the 64-bit sum of values
 template <int P>
-__device__ __forceinline__ double lanes_norm(const LaneArg &a, float k, const uint64_t *__restrict__ part, uint32_t parts)
+__device__ __forceinline__ uint64_t lanes_join(bool exact, uint64_t x, uint64_t y)
 {
-    if (lanes_exact(a, k)) {
-        uint64_t t = 0;
-        for (uint32_t i = lane_id(); i < parts; i += 64)
-            t = P == kPInf ? max(t, part[i]) : t + part[i];
+    if (exact)
+        return P == kPInf ? max(x, y) : x + y;
+    Acc<P> a, b;
+    a.set(__longlong_as_double((long long)x));
+    b.set(__longlong_as_double((long long)y));
+    a.join(b);
+    return (uint64_t)__double_as_longlong(a.value());
+}
+
+template <int P>
+__device__ __forceinline__ uint64_t lanes_wave(bool exact, uint64_t x)
+{
 #pragma unroll
-        for (int m = 32; m; m >>= 1) {
-            const uint64_t o = __shfl_xor(t, m, 64);
-            t = P == kPInf ? max(t, o) : t + o;
+    for (int m = 32; m; m >>= 1)
+        x = lanes_join<P>(exact, x, __shfl_xor(x, m, 64));
+    return x;
+}
+
+template <int P>
+__device__ __forceinline__ double lanes_root(const LaneArg &a, float k, bool exact, uint64_t t)
+{
+    if (!exact)
+        return root_of(P, __longlong_as_double((long long)t));
+    if (P == kPInf)
+        return fabs((double)(k * (float)t * a.alpha));
+    const double step = fabs((double)k * (double)a.alpha);
+    return P == 2 ? step * sqrt((double)t) : step * (double)t;
+}
+
+// four words' lanes l0 <= l < l1 at flat elements l M + i .. + 3; CHECK: those below n
+template <int P, bool CHECK>
+__device__ __forceinline__ uint32_t quad_sum(const LaneArg &a, uint4 wd, uint64_t i, uint32_t l0, uint32_t l1, uint32_t mask,
+                                             uint32_t sum)
+{
+    for (uint32_t l = l0; l < l1; ++l) {
+        const uint32_t we[4] = {wd.x, wd.y, wd.z, wd.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            int32_t q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;  // |q| < 2^14
+            if (CHECK && (uint64_t)l * a.M + i + e >= a.n)
+                q = 0;
+            if (P == 2) {
+                sum += (uint32_t)__mul24(q, q);
+            } else {
+                const uint32_t m = (uint32_t)(q < 0 ? -q : q);
+                sum = P == kPInf ? max(sum, m) : sum + m;
+            }
         }
-        if (P == kPInf)
-            return fabs((double)(k * (float)t * a.alpha));
-        const double step = fabs((double)k * (double)a.alpha);
-        return P == 2 ? step * sqrt((double)t) : step * (double)t;
     }
-    return root_of(P, wave_total<P>(reinterpret_cast<const double *>(part), parts));
+    return sum;
+}
+
+// the block's share of the norm of the words, valid in thread 0
+template <int P>
+__device__ __forceinline__ uint64_t block_lanes(const LaneArg &a, float k, bool exact)
+{
+    __shared__ uint64_t part[kNormThreads / 64];
+    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u;
+    const uint32_t full = (uint32_t)min(a.M ? a.n / a.M : 0, (uint64_t)a.L);  // planes that are full to the end
+    const uint64_t quads = a.M >> 2, stride = (uint64_t)gridDim.x * kNormThreads;
+    const uint4 *words = reinterpret_cast<const uint4 *>(a.words);
+    uint64_t t = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x, sum = 0;
+    if (exact) {
+        // w <= 14: a quad's sum is at most L * 4 * 2^(2w) <= 2^31
+        auto add = [&](uint4 wd, uint64_t i) {
+            uint32_t q = quad_sum<P, false>(a, wd, i, 0, full, mask, 0u);
+            q = quad_sum<P, true>(a, wd, i, full, a.L, mask, q);
+            sum = lanes_join<P>(true, sum, (uint64_t)q);
+        };
+        constexpr int U = 4;
+        for (; t + (U - 1) * stride < quads; t += U * stride) {
+            uint4 wd[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                wd[u] = words[t + u * stride];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                add(wd[u], 4 * (t + u * stride));
+        }
+        for (; t < quads; t += stride)
+            add(words[t], 4 * t);
+    } else {
+        Acc<P> real;
+        for (; t < quads; t += stride) {
+            const uint4 wd = words[t];
+            const uint32_t we[4] = {wd.x, wd.y, wd.z, wd.w};
+            for (uint32_t l = 0; l < a.L; ++l)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int32_t q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
+                    if ((uint64_t)l * a.M + 4 * t + e < a.n)
+                        real.add(k * (float)q * a.alpha);
+                }
+        }
+        sum = (uint64_t)__double_as_longlong(real.value());
+    }
+    sum = lanes_wave<P>(exact, sum);
+    if (lane_id() == 0)
+        part[wave_id()] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (unsigned w = 1; w < kNormThreads / 64; ++w)
+            sum = lanes_join<P>(exact, sum, part[w]);
+    return sum;
 }
 
 template <int P>
 __global__ __launch_bounds__(kNormThreads) void k_lane_norm(LaneArg a, uint64_t *__restrict__ part)
 {
-    __shared__ uint64_t sint[kNormThreads / 64];
     const float k = *a.norm / a.s;
-    const bool exact = lanes_exact(a, k);
-    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u;
-    const uint64_t quads = a.M >> 2, stride = (uint64_t)gridDim.x * kNormThreads;
-    uint64_t sum = 0;
-    Acc<P> real;
-    for (uint64_t t = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x; t < quads; t += stride) {
-        const uint4 wd = *reinterpret_cast<const uint4 *>(a.words + 4 * t);
-        uint32_t we[4] = {wd.x, wd.y, wd.z, wd.w};
-        uint32_t quad = 0;  // w <= 14: at most L * 4 * 2^(2w) <= 2^31
-        for (uint32_t l = 0; l < a.L; ++l) {
-            const uint64_t i0 = (uint64_t)l * a.M + 4 * t;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int32_t q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
-                const bool in = i0 + e < a.n;
-                if (exact) {
-                    const uint32_t m = in ? (uint32_t)(q < 0 ? -q : q) : 0u;
-                    quad = P == kPInf ? max(quad, m) : P == 2 ? quad + m * m : quad + m;
-                } else if (in) {
-                    real.add(k * (float)q * a.alpha);
-                }
-            }
-        }
-        sum = P == kPInf ? max(sum, (uint64_t)quad) : sum + quad;
-    }
-    if (exact) {
-#pragma unroll
-        for (int m = 32; m; m >>= 1) {
-            const uint64_t o = __shfl_xor(sum, m, 64);
-            sum = P == kPInf ? max(sum, o) : sum + o;
-        }
-    } else {
-        wave_join(real);
-        sum = (uint64_t)__double_as_longlong(real.value());
-    }
-    if (lane_id() == 0)
-        sint[wave_id()] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (unsigned w = 1; w < kNormThreads / 64; ++w) {
-            if (exact) {
-                sum = P == kPInf ? max(sum, sint[w]) : sum + sint[w];
-            } else {
-                Acc<P> o;
-                o.set(__longlong_as_double((long long)sint[w]));
-                real.join(o);
-            }
-        }
-        part[blockIdx.x] = exact ? sum : (uint64_t)__double_as_longlong(real.value());
-    }
+    const uint64_t sum = block_lanes<P>(a, k, lanes_exact(a, k));
+    if (threadIdx.x == 0)
+        part[blockIdx.x] = sum;
 }
 
 // the lane's quad v of flat elements i .. i + 3, those inside [a, b), to the
@@ -494,17 +617,60 @@ __device__ __forceinline__ void store_quad(uint64_t base, uint64_t start, uint64
             y[i + e - start] = Elem<T>::down(v[e]);
 }
 
-// A wave takes 256 kQuads consecutive words, L ranges of as many flat elements
-template <bool LDS>
-__global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradArg dst, int p, double max_norm,
+// Tile t: 256 kQuads consecutive words, L ranges of as many flat elements
+constexpr int kQuads = 2;
+__device__ __forceinline__ void decode_tile(const LaneArg &a, const GradRec *rd, uint32_t count, uint64_t t, float k, float c)
+{
+    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u, lane = lane_id();
+    const uint64_t j0 = t * (256 * kQuads), j1 = min(j0 + 256 * kQuads, a.M);
+    uint4 wd[kQuads];
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        const uint64_t j = j0 + 256 * q + 4 * lane;  // M is a multiple of 4: a quad is in or out
+        wd[q] = j < j1 ? *reinterpret_cast<const uint4 *>(a.words + j) : make_uint4(0, 0, 0, 0);
+    }
+    for (uint32_t l = 0; l < a.L; ++l) {
+        const uint64_t lo = (uint64_t)l * a.M + j0, hi = min((uint64_t)l * a.M + j1, a.n);
+        if (lo >= hi)
+            break;
+        grad_walk(rd, count, lo, hi, [&](uint32_t, uint32_t type, uint64_t base, uint64_t start, uint64_t pa, uint64_t pb) {
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                if (lo + 256 * q >= pb || lo + 256 * (q + 1) <= pa)
+                    continue;
+                const uint32_t we[4] = {wd[q].x, wd[q].y, wd[q].z, wd[q].w};
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int32_t Q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
+                    const float d = k * (float)Q;
+                    v[e] = d * a.alpha * c;
+                }
+                const uint64_t i = lo + 256 * q + 4 * lane;
+                if (type == kTF32)
+                    store_quad<float>(base, start, pa, pb, i, v);
+                else if (type == kTBF16)
+                    store_quad<__bf16>(base, start, pa, pb, i, v);
+                else
+                    store_quad<_Float16>(base, start, pa, pb, i, v);
+            }
+        });
+    }
+}
+
+__host__ __device__ __forceinline__ uint64_t decode_tiles(uint64_t M) { return (M + 256 * kQuads - 1) / (256 * kQuads); }
+
+template <int P, bool LDS>
+__global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradArg dst, double max_norm,
                                                                const uint64_t *__restrict__ part, uint32_t parts,
                                                                float *__restrict__ norm)
 {
-    constexpr int kQuads = 2;
     const float k = *a.norm / a.s;
-    const double N = p == 2   ? lanes_norm<2>(a, k, part, parts)
-                     : p == 1 ? lanes_norm<1>(a, k, part, parts)
-                              : lanes_norm<kPInf>(a, k, part, parts);
+    const bool exact = lanes_exact(a, k);
+    uint64_t sum = 0;  // the bits of 0.0 as well
+    for (uint32_t i = lane_id(); i < parts; i += 64)
+        sum = lanes_join<P>(exact, sum, part[i]);
+    const double N = lanes_root<P>(a, k, exact, lanes_wave<P>(exact, sum));
     const float c = clip_coef(N, max_norm);
     if (blockIdx.x == 0 && threadIdx.x == 0)
         *norm = (float)N;
@@ -514,45 +680,31 @@ __global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradAr
         stage_table(dst, sd);
         __syncthreads();
     }
-    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u, lane = lane_id();
-    const uint64_t tiles = (a.M + 256 * kQuads - 1) / (256 * kQuads), waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
-    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves) {
-        const uint64_t j0 = t * (256 * kQuads), j1 = min(j0 + 256 * kQuads, a.M);
-        uint4 wd[kQuads];
-#pragma unroll
-        for (int q = 0; q < kQuads; ++q) {
-            const uint64_t j = j0 + 256 * q + 4 * lane;  // M is a multiple of 4: a quad is in or out
-            wd[q] = j < j1 ? *reinterpret_cast<const uint4 *>(a.words + j) : make_uint4(0, 0, 0, 0);
-        }
-        for (uint32_t l = 0; l < a.L; ++l) {
-            const uint64_t lo = (uint64_t)l * a.M + j0, hi = min((uint64_t)l * a.M + j1, a.n);
-            if (lo >= hi)
-                break;
-            grad_walk(rd, dst.count, lo, hi,
-                      [&](uint32_t, uint32_t type, uint64_t base, uint64_t start, uint64_t pa, uint64_t pb) {
-#pragma unroll
-                          for (int q = 0; q < kQuads; ++q) {
-                              if (lo + 256 * q >= pb || lo + 256 * (q + 1) <= pa)
-                                  continue;
-                              const uint32_t we[4] = {wd[q].x, wd[q].y, wd[q].z, wd[q].w};
-                              float v[4];
-#pragma unroll
-                              for (int e = 0; e < 4; ++e) {
-                                  const int32_t Q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
-                                  const float d = k * (float)Q;
-                                  v[e] = d * a.alpha * c;
-                              }
-                              const uint64_t i = lo + 256 * q + 4 * lane;
-                              if (type == kTF32)
-                                  store_quad<float>(base, start, pa, pb, i, v);
-                              else if (type == kTBF16)
-                                  store_quad<__bf16>(base, start, pa, pb, i, v);
-                              else
-                                  store_quad<_Float16>(base, start, pa, pb, i, v);
-                          }
-                      });
-        }
+    const uint64_t tiles = decode_tiles(a.M), waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
+    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves)
+        decode_tile(a, rd, dst.count, tiles - 1 - t, k, c);
+}
+
+// both passes in one block
+template <int P>
+__global__ __launch_bounds__(kNormThreads) void k_decode_clip_one(LaneArg a, GradArg dst, double max_norm,
+                                                                  float *__restrict__ norm)
+{
+    __shared__ GradRec sd[kLdsRecs + 1];
+    __shared__ float sc;
+    const float k = *a.norm / a.s;
+    const bool exact = lanes_exact(a, k);
+    if (a.n)
+        stage_table(dst, sd);  // ahead of block_lanes's barrier
+    const uint64_t sum = block_lanes<P>(a, k, exact);
+    if (threadIdx.x == 0) {
+        const double N = lanes_root<P>(a, k, exact, sum);
+        sc = clip_coef(N, max_norm);
+        *norm = (float)N;
     }
+    __syncthreads();
+    for (uint64_t t = wave_id(), tiles = decode_tiles(a.M); t < tiles; t += kNormThreads / 64)
+        decode_tile(a, sd, dst.count, t, k, sc);
 }
 
 // ---------------------------------------------------------------------------
@@ -599,7 +751,7 @@ static int check_output(const gc_grads *g, const char *what)
     return GC_OK;
 }
 
-// whether [lo, hi) meets a tensor of the (disjoint) table; *at its index
+// whether [lo, hi) meets a tensor of the (disjoint) table; *at the first one's index
 static bool meets(const gc_grads *g, Span x, uint64_t *at)
 {
     if (x.lo >= x.hi)
@@ -618,6 +770,34 @@ static bool meets(const gc_grads *g, Span x, uint64_t *at)
     const Span y = span_of(g, g->order[a]);
     *at = g->order[a];
     return y.lo < y.hi && y.lo < x.hi;
+}
+
+// A tensor may be clipped onto itself; any other input that meets an output
+// could be read after it is written.  Both lists by address: one pass.
+static int check_apart(const gc_grads *src, const gc_grads *dst, const char *what)
+{
+    uint64_t j = 0;
+    for (uint64_t i = 0; i < src->count; ++i) {
+        const uint32_t s = src->order[i];
+        const Span x = span_of(src, s);
+        if (x.lo >= x.hi)
+            break;
+        while (j < dst->count) {  // the first output that ends behind x.lo (inputs are by their starts)
+            const Span y = span_of(dst, dst->order[j]);
+            if (y.lo >= y.hi || y.hi > x.lo)
+                break;
+            ++j;
+        }
+        for (uint64_t k = j; k < dst->count; ++k) {
+            const uint32_t d = dst->order[k];
+            const Span y = span_of(dst, d);
+            if (y.lo >= y.hi || y.lo >= x.hi)
+                break;
+            GC_REQUIRE(s == d && src->host_rec[2 * s] == dst->host_rec[2 * s],
+                       "%s: input tensor %u shares memory with output tensor %u", what, s, d);
+        }
+    }
+    return GC_OK;
 }
 
 static int check_p(uint32_t p, const char *what)
@@ -643,33 +823,38 @@ static unsigned norm_grid(uint64_t n)
     return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
 }
 
-// the partials of the norm -> their number
+// whether one block does both passes of a clip of n elements
+static bool one_block(uint64_t n, uint64_t count) { return n <= kOneTiles * kTile && count <= kLdsRecs; }
+
+// f(p as a constant)
+template <class F>
+static void with_p(uint32_t p, F f)
+{
+    if (p == 2)
+        f(std::integral_constant<int, 2>());
+    else if (p == 1)
+        f(std::integral_constant<int, 1>());
+    else
+        f(std::integral_constant<int, kPInf>());
+}
+
 template <bool EACH, bool PEAK>
-static void launch_norm(const gc_grads *g, uint32_t p, void *ws, hipStream_t st)
+static void launch_norm(const gc_grads *g, uint32_t p, void *ws, double *total, float *norm, float *each, hipStream_t st)
 {
     const GradArg a = arg_of(g);
-    const unsigned grid = norm_grid(g->n);
+    const dim3 grid(norm_grid(g->n)), block(kNormThreads);
     char *w = static_cast<char *>(ws);
     double *part = reinterpret_cast<double *>(w);
     uint32_t *peak = reinterpret_cast<uint32_t *>(w + kWsPeak);
     double *slots = reinterpret_cast<double *>(w + kWsSlots);
-    const bool lds = g->count <= kLdsRecs;
-#define GC_GN(P_)                                                                                                   \
-    do {                                                                                                            \
-        if (lds)                                                                                                    \
-            hipLaunchKernelGGL((k_grad_norm<P_, EACH, PEAK, true>), dim3(grid), dim3(kNormThreads), 0, st, a, g->n, \
-                               part, peak, slots);                                                                  \
-        else                                                                                                        \
-            hipLaunchKernelGGL((k_grad_norm<P_, EACH, PEAK, false>), dim3(grid), dim3(kNormThreads), 0, st, a,      \
-                               g->n, part, peak, slots);                                                            \
-    } while (0)
-    if (p == 2)
-        GC_GN(2);
-    else if (p == 1)
-        GC_GN(1);
-    else
-        GC_GN(kPInf);
-#undef GC_GN
+    with_p(p, [&](auto P) {
+        if (g->count <= kLdsRecs)
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, part, peak, slots, total,
+                               norm, each);
+        else
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, part, peak, slots, total,
+                               norm, each);
+    });
 }
 
 static unsigned scale_grid(uint64_t tiles)
@@ -766,14 +951,19 @@ int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, 
     GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
     hipStream_t st = as_stream(stream);
     if (each)
-        launch_norm<true, false>(grads, p, workspace, st);
+        launch_norm<true, false>(grads, p, workspace, total, norm, each, st);
     else
-        launch_norm<false, false>(grads, p, workspace, st);
-    char *w = static_cast<char *>(workspace);
-    const unsigned blocks = 1 + (each ? (unsigned)grads->count : 0u);
-    hipLaunchKernelGGL(k_grad_finish, dim3(blocks), dim3(kScaleThreads), 0, st, arg_of(grads), (int)p,
-                       reinterpret_cast<const double *>(w), norm_grid(grads->n),
-                       reinterpret_cast<const double *>(w + kWsSlots), total, norm, each);
+        launch_norm<false, false>(grads, p, workspace, total, norm, each, st);
+    const unsigned parts = norm_grid(grads->n);
+    if (parts > 1) {
+        const char *w = static_cast<const char *>(workspace);
+        const dim3 grid(1 + (each ? (unsigned)grads->count : 0u));
+        with_p(p, [&](auto P) {
+            hipLaunchKernelGGL(k_grad_finish<P()>, grid, dim3(kNormThreads), 0, st, arg_of(grads),
+                               reinterpret_cast<const double *>(w), parts, reinterpret_cast<const double *>(w + kWsSlots),
+                               total, norm, each);
+        });
+    }
     return launch_status(what);
 }
 
@@ -784,8 +974,10 @@ int gc_grad_norm_root(const double *total, uint32_t p, float *norm, gc_stream_t 
     if ((rc = check_p(p, what)))
         return rc;
     GC_REQUIRE(total && norm, "%s: null pointer", what);
-    hipLaunchKernelGGL(k_grad_finish, dim3(1), dim3(kScaleThreads), 0, as_stream(stream), GradArg{nullptr, 0}, (int)p,
-                       total, 1u, nullptr, nullptr, norm, nullptr);
+    with_p(p, [&](auto P) {
+        hipLaunchKernelGGL(k_grad_finish<P()>, dim3(1), dim3(64), 0, as_stream(stream), GradArg{nullptr, 0}, total, 1u,
+                           nullptr, nullptr, norm, nullptr);
+    });
     return launch_status(what);
 }
 
@@ -804,20 +996,20 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
         GC_REQUIRE(src->host_rec[2 * s + 1] == dst->host_rec[2 * s + 1], "%s: the two lists differ in tensor sizes", what);
         same &= src->host_rec[2 * s] == dst->host_rec[2 * s];
     }
-    for (uint64_t s = 0; !same && s < src->count; ++s) {
-        uint64_t at = 0;
-        const Span x = span_of(src, s);
-        // a tensor may be clipped onto itself; any other meeting would be read after it is written
-        if (meets(dst, x, &at))
-            GC_REQUIRE(at == s && src->host_rec[2 * s] == dst->host_rec[2 * s],
-                       "%s: input tensor %llu shares memory with output tensor %llu", what, (unsigned long long)s,
-                       (unsigned long long)at);
-    }
+    if (!same && (rc = check_apart(src, dst, what)))
+        return rc;
     GC_REQUIRE(total || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0),
                "%s: null or misaligned workspace", what);
     hipStream_t st = as_stream(stream);
+    if (!total && one_block(src->n, src->count)) {
+        with_p(p, [&](auto P) {
+            hipLaunchKernelGGL((k_grad_clip_one<P(), false>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), arg_of(dst),
+                               nullptr, src->n, max_norm, same, norm, nullptr);
+        });
+        return launch_status(what);
+    }
     if (!total)
-        launch_norm<false, false>(src, p, workspace, st);
+        launch_norm<false, false>(src, p, workspace, nullptr, nullptr, nullptr, st);
     const double *part = total ? total : static_cast<const double *>(workspace);
     const unsigned parts = total ? 1u : norm_grid(src->n);
     const unsigned grid = scale_grid((src->n + kTile - 1) / kTile);
@@ -848,7 +1040,14 @@ int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double ma
                    (unsigned long long)s);
     }
     hipStream_t st = as_stream(stream);
-    launch_norm<false, true>(src, p, workspace, st);
+    if (one_block(src->n, src->count)) {
+        with_p(p, [&](auto P) {
+            hipLaunchKernelGGL((k_grad_clip_one<P(), true>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), GradArg{}, flat,
+                               src->n, max_norm, false, norm, peak);
+        });
+        return launch_status(what);
+    }
+    launch_norm<false, true>(src, p, workspace, nullptr, nullptr, nullptr, st);
     const char *w = static_cast<const char *>(workspace);
     const unsigned grid = scale_grid((src->n + kTile - 1) / kTile), parts = norm_grid(src->n);
     const GradArg a = arg_of(src);
@@ -890,19 +1089,21 @@ int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, ui
     const unsigned parts =
         (unsigned)std::min<uint64_t>(std::max<uint64_t>((quads + kNormThreads - 1) / kNormThreads, 1), kNormGrid);
     uint64_t *part = static_cast<uint64_t *>(workspace);
-    const unsigned grid = scale_grid((lanes->plane_words + 511) / 512);
-    if (p == 2)
-        hipLaunchKernelGGL(k_lane_norm<2>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
-    else if (p == 1)
-        hipLaunchKernelGGL(k_lane_norm<1>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
-    else
-        hipLaunchKernelGGL(k_lane_norm<kPInf>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
-    if (dst->count <= kLdsRecs)
-        hipLaunchKernelGGL((k_decode_clip<true>), dim3(grid), dim3(kScaleThreads), 0, st, a, arg_of(dst), (int)p, max_norm,
-                           part, parts, total_norm);
-    else
-        hipLaunchKernelGGL((k_decode_clip<false>), dim3(grid), dim3(kScaleThreads), 0, st, a, arg_of(dst), (int)p, max_norm,
-                           part, parts, total_norm);
+    const GradArg d = arg_of(dst);
+    const dim3 grid(scale_grid(decode_tiles(lanes->plane_words)));
+    with_p(p, [&](auto P) {
+        if (one_block(n, dst->count)) {
+            hipLaunchKernelGGL(k_decode_clip_one<P()>, dim3(1), dim3(kNormThreads), 0, st, a, d, max_norm, total_norm);
+            return;
+        }
+        hipLaunchKernelGGL(k_lane_norm<P()>, dim3(parts), dim3(kNormThreads), 0, st, a, part);
+        if (dst->count <= kLdsRecs)
+            hipLaunchKernelGGL((k_decode_clip<P(), true>), grid, dim3(kScaleThreads), 0, st, a, d, max_norm, part, parts,
+                               total_norm);
+        else
+            hipLaunchKernelGGL((k_decode_clip<P(), false>), grid, dim3(kScaleThreads), 0, st, a, d, max_norm, part, parts,
+                               total_norm);
+    });
     return launch_status(what);
 }
 

@@ -29,16 +29,17 @@ from __future__ import annotations
 import ctypes as C
 import math
 import numbers
+import operator
 
 import numpy as np
 import torch
 import torch.distributed as dist
 
 from . import _lib
-from ._lib import check
-from .codec import _dev, _f32, _p, _stream, norm_tensor, qsgd_layout
+from .codec import _dev, _raw_stream, norm_tensor, qsgd_layout
 
 _TYPE = {torch.float32: _lib.GC_F32, torch.float16: _lib.GC_F16, torch.bfloat16: _lib.GC_BF16}
+_dtype_of, _grad_of = operator.attrgetter("dtype"), operator.attrgetter("grad")
 
 
 def _refuse(msg: str):
@@ -47,11 +48,13 @@ def _refuse(msg: str):
 
 def _norm_code(norm_type) -> int:
     p = float(norm_type)
+    if p == 2.0:
+        return 2
     if p == math.inf:
         return _lib.GC_NORM_INF
-    if p not in (1.0, 2.0):
+    if p != 1.0:
         _refuse(f"norm_type must be 1, 2 or inf, got {norm_type}")
-    return int(p)
+    return 1
 
 
 def _limit(max_norm) -> float:
@@ -60,19 +63,17 @@ def _limit(max_norm) -> float:
     return float(max_norm)
 
 
-class _on:
-    """Makes `device` the current one for a launch, where it is not already."""
-
-    def __init__(self, device):
-        self._ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+def _call(name: str, device, *args):
+    """One entry point on `device` and its current stream (the last argument)."""
+    fn = getattr(_lib.load(), name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc < 0:
+        raise _lib.GCodecError(rc, f"{name}: {_lib.last_error()}")
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -106,7 +107,7 @@ class Grads:
             _refuse("Grads: made under graph capture; make the table before it")
         rec = torch.from_numpy(self._host.view(np.int64))
         self._rec = rec.to(self.device)  # complete when this returns, whatever stream reads it
-        self._home = torch.cuda.current_stream(self.device)
+        self._home = _raw_stream(self.device.index)
         self.struct.rec = self._rec.data_ptr()
         self._keep = [t.untyped_storage() for t in tensors]
 
@@ -116,26 +117,27 @@ class Grads:
         self = cls.__new__(cls)
         self._build(tensors, ordered)
         self._rec = torch.empty(self._host.size, dtype=torch.int64, device=self.device)
-        with _on(self.device):
-            check(_lib.load().gc_grads_fill(C.byref(self.struct), _p(self._rec), _stream(self.device)), "gc_grads_fill")
         self._home = None
         self.struct.rec = self._rec.data_ptr()
+        _call("gc_grads_fill", self.device, self._ref, self.struct.rec)
         return self
 
     def _build(self, tensors, ordered=True):
         """ordered: element i of a tensor is its i-th in row-major order (else any dense order does)"""
         if not tensors:
             _refuse("Grads: empty tensor list")
-        for t in tensors:
-            if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
-                _refuse(f"Grads: not a dense tensor ({type(t).__name__})")
-        self.device = dev = _dev(tensors[0])
-        if len(set(map(torch.Tensor.get_device, tensors))) != 1:
+        try:
+            devices = set(map(torch.Tensor.get_device, tensors))
+            dtypes = set(map(_dtype_of, tensors))
+            contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+        except (TypeError, RuntimeError):  # not a tensor; a sparse one has no strides
+            _refuse("Grads: not a list of dense tensors")
+        self.device = _dev(tensors[0])
+        if len(devices) != 1:
             _refuse("Grads: the tensors are on different devices")
-        types = list(map(_TYPE.get, [t.dtype for t in tensors]))
-        if None in types:
-            _refuse(f"Grads: {tensors[types.index(None)].dtype} is not float32, float16 or bfloat16")
-        if not all(map(torch.Tensor.is_contiguous, tensors)):
+        if not dtypes <= _TYPE.keys():
+            _refuse(f"Grads: {(dtypes - _TYPE.keys()).pop()} is not float32, float16 or bfloat16")
+        if not contiguous:
             bad = [i for i, t in enumerate(tensors) if not (t.is_contiguous() if ordered else _dense(t))]
             if bad:
                 t = tensors[bad[0]]
@@ -143,23 +145,35 @@ class Grads:
                         f"strides {t.stride()})")
         lib = _lib.load()
         self.count = count = len(tensors)
-        sizes = np.fromiter(map(torch.Tensor.numel, tensors), dtype=np.uint64, count=count)
-        ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), dtype=np.uint64, count=count)
-        kinds = np.fromiter(types, dtype=np.uint32, count=count)
+        sizes = (C.c_uint64 * count)(*map(torch.Tensor.numel, tensors))
+        ptrs = (C.c_uint64 * count)(*map(torch.Tensor.data_ptr, tensors))
+        if len(dtypes) == 1:
+            kinds = (C.c_uint32 * count)(*(_TYPE[dtypes.pop()],) * count)
+        else:
+            kinds = (C.c_uint32 * count)(*map(_TYPE.__getitem__, map(_dtype_of, tensors)))
         self._host = np.empty(2 * (count + 1), dtype=np.uint64)
         self._order = np.empty(count, dtype=np.uint32)
         self.struct = _lib.gc_grads()
-        check(lib.gc_grads_plan(sizes.ctypes.data, ptrs.ctypes.data, kinds.ctypes.data, count, self._host.ctypes.data,
-                                self._order.ctypes.data, C.byref(self.struct)), "gc_grads_plan")
+        self._ref = C.byref(self.struct)
+        rc = lib.gc_grads_plan(sizes, ptrs, kinds, count, self._host.ctypes.data, self._order.ctypes.data, self._ref)
+        if rc < 0:
+            raise _lib.GCodecError(rc, f"gc_grads_plan: {_lib.last_error()}")
         self.n = int(self.struct.n)
+        self._ws = lib.gc_grad_workspace_size(self.n, count, 0)
 
     def _use(self):
-        """Tells the allocator of a stream other than the one the table was made on."""
-        if self._home is not None and not torch.cuda.is_current_stream_capturing():
-            now = torch.cuda.current_stream(self.device)
-            if now != self._home:
-                self._rec.record_stream(now)
-        return C.byref(self.struct)
+        """The table for a launch; the allocator is told of a stream other than the one the table was made on."""
+        if self._home is not None and _raw_stream(self.device.index) != self._home:
+            if not torch.cuda.is_current_stream_capturing():
+                self._rec.record_stream(torch.cuda.current_stream(self.device))
+        return self._ref
+
+    def _workspace(self, each: bool = False) -> torch.Tensor:
+        size = _lib.load().gc_grad_workspace_size(self.n, self.count, 1) if each else self._ws
+        return torch.empty(size, dtype=torch.uint8, device=self.device)
+
+    def _scalar(self, dtype=torch.float32) -> torch.Tensor:
+        return torch.empty((), dtype=dtype, device=self.device)
 
 
 def _table(grads, ordered=True) -> Grads:
@@ -168,15 +182,6 @@ def _table(grads, ordered=True) -> Grads:
     if isinstance(grads, torch.Tensor):
         grads = [grads]
     return Grads._of_call(list(grads), ordered)
-
-
-def _workspace(g: Grads, each: bool = False) -> torch.Tensor:
-    size = _lib.load().gc_grad_workspace_size(g.n, g.count, int(each))
-    return torch.empty(size, dtype=torch.uint8, device=g.device)
-
-
-def _scalar(g: Grads, dtype=torch.float32) -> torch.Tensor:
-    return torch.empty((), dtype=dtype, device=g.device)
 
 
 def _sum_ranks(total: torch.Tensor, code: int, group) -> torch.Tensor:
@@ -199,50 +204,49 @@ def _finite(norm: torch.Tensor, what: str):
         raise RuntimeError(f"{what}: the total norm of the gradients is {float(norm)}, which is not finite")
 
 
-@torch.no_grad()
+def _norm_into(g: Grads, code: int, norm, each=None, total=None):
+    ws = g._workspace(each is not None)
+    _call("gc_grad_norm", g.device, g._use(), code, total.data_ptr() if total is not None else None,
+          norm.data_ptr() if norm is not None else None, each.data_ptr() if each is not None else None, ws.data_ptr())
+
+
 def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False, error_if_nonfinite: bool = False, group=None):
     """The norm of all gradients together, a float32 scalar tensor; with
     per_tensor=True (norm, norms), `norms` a float32 tensor of each tensor's own
     (with a group: of this rank's part).  No gradients at all have norm 0."""
     code = _norm_code(norm_type)
     g = _table(grads, ordered=False)
-    lib = _lib.load()
-    with _on(g.device):
-        norm = _scalar(g)
-        each = torch.empty(g.count, dtype=torch.float32, device=g.device) if per_tensor else None
-        total = _scalar(g, torch.float64) if group is not None else None
-        check(lib.gc_grad_norm(g._use(), code, _p(total), _p(norm), _p(each), _p(_workspace(g, per_tensor)),
-                               _stream(g.device)), "gc_grad_norm")
-        if group is not None:
-            _sum_ranks(total, code, group)
-            check(lib.gc_grad_norm_root(_p(total), code, _p(norm), _stream(g.device)), "gc_grad_norm_root")
+    norm = g._scalar()
+    each = torch.empty(g.count, dtype=torch.float32, device=g.device) if per_tensor else None
+    total = g._scalar(torch.float64) if group is not None else None
+    _norm_into(g, code, norm, each, total)
+    if group is not None:
+        _sum_ranks(total, code, group)
+        _call("gc_grad_norm_root", g.device, total.data_ptr(), code, norm.data_ptr())
     if error_if_nonfinite:
         _finite(norm, "grad_norm")
     return (norm, each) if per_tensor else norm
 
 
 def _clip(src: Grads, dst: Grads, max_norm: float, code: int, error_if_nonfinite: bool, group, what: str):
-    lib = _lib.load()
     if src.device != dst.device:
         _refuse(f"{what}: gradients on {src.device}, outputs on {dst.device}")
-    with _on(src.device):
-        norm = _scalar(src)
-        total = None
-        if group is not None or error_if_nonfinite:
-            total = _scalar(src, torch.float64)
-            check(lib.gc_grad_norm(src._use(), code, _p(total), None, None, _p(_workspace(src)), _stream(src.device)),
-                  "gc_grad_norm")
-            if group is not None:
-                _sum_ranks(total, code, group)
-            if error_if_nonfinite:  # before anything is written
-                check(lib.gc_grad_norm_root(_p(total), code, _p(norm), _stream(src.device)), "gc_grad_norm_root")
-                _finite(norm, what)
-        check(lib.gc_grad_clip(src._use(), dst._use(), code, max_norm, _p(total), _p(norm), _p(_workspace(src)),
-                               _stream(src.device)), "gc_grad_clip")
+    norm = src._scalar()
+    total = None
+    if group is not None or error_if_nonfinite:
+        total = src._scalar(torch.float64)
+        _norm_into(src, code, None, total=total)
+        if group is not None:
+            _sum_ranks(total, code, group)
+        if error_if_nonfinite:  # before anything is written
+            _call("gc_grad_norm_root", src.device, total.data_ptr(), code, norm.data_ptr())
+            _finite(norm, what)
+    ws = src._workspace()
+    _call("gc_grad_clip", src.device, src._use(), dst._use(), code, max_norm,
+          total.data_ptr() if total is not None else None, norm.data_ptr(), ws.data_ptr())
     return norm
 
 
-@torch.no_grad()
 def clip_grads(grads, out, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, group=None):
     """out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), two lists of the same
     tensor sizes (their types may differ); -> the norm before clipping.  A
@@ -254,14 +258,13 @@ def clip_grads(grads, out, max_norm: float, norm_type: float = 2.0, error_if_non
     return _clip(src, dst, max_norm, code, error_if_nonfinite, group, "clip_grads")
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, group=None):
     """Clips the gradients of `parameters` in place; -> their norm before it (a
     float32 scalar tensor, 0 without any gradient).  As
     torch.nn.utils.clip_grad_norm_, with the norm held in 64 bits."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [g for g in (p.grad for p in parameters) if g is not None]
+    grads = [g for g in map(_grad_of, parameters) if g is not None]
     if not grads:
         dev = parameters[0].device if parameters else None
         norm = torch.zeros((), dtype=torch.float64, device=dev)
@@ -275,30 +278,30 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         return norm
     src = _table(grads, ordered=False)
     norm = _clip(src, src, max_norm, code, error_if_nonfinite, group, "clip_grad_norm_")
-    torch.autograd.graph.increment_version([g for g in grads if not g.is_inference()])
+    if any(map(torch.Tensor.is_inference, grads)):  # these have no version
+        grads = [g for g in grads if not g.is_inference()]
+    torch.autograd.graph.increment_version(grads)
     return norm
 
 
-@torch.no_grad()
 def flatten_clip(grads, max_norm: float, norm_type: float = 2.0, flat=None):
     """-> (flat, peak, norm): the clipped gradients end to end in one float32
     bucket, its max-norm (as segments_flatten_absmax: what qsgd_encode scales
     by), and the gradients' norm before clipping."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     g = _table(grads)
-    with _on(g.device):
-        if flat is None:
-            flat = torch.empty(g.n, dtype=torch.float32, device=g.device)
-        elif flat.device != g.device or flat.numel() != g.n or not flat.is_contiguous():
-            _refuse(f"flatten_clip: flat must be contiguous, {g.n} elements on {g.device}")
-        peak = torch.empty(1, dtype=torch.float32, device=g.device)
-        norm = _scalar(g)
-        check(_lib.load().gc_grad_flatten_clip(g._use(), _p(_f32(flat, "flatten_clip")), code, max_norm, _p(peak),
-                                               _p(norm), _p(_workspace(g)), _stream(g.device)), "gc_grad_flatten_clip")
+    if flat is None:
+        flat = torch.empty(g.n, dtype=torch.float32, device=g.device)
+    elif flat.device != g.device or flat.dtype != torch.float32 or flat.numel() != g.n or not flat.is_contiguous():
+        _refuse(f"flatten_clip: flat must be contiguous float32, {g.n} elements on {g.device}")
+    peak = torch.empty(1, dtype=torch.float32, device=g.device)
+    norm = g._scalar()
+    ws = g._workspace()
+    _call("gc_grad_flatten_clip", g.device, g._use(), flat.data_ptr(), code, max_norm, peak.data_ptr(), norm.data_ptr(),
+          ws.data_ptr())
     return flat, peak, norm
 
 
-@torch.no_grad()
 def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: float = 2.0, world: int = 1,
                      alpha: float = 1.0, lanes=None):
     """qsgd_decode of the packed words (summed over `world` ranks) times alpha into
@@ -314,12 +317,11 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     lanes = lanes or qsgd_layout(g.n, bits, world)
     if words.numel() < lanes.plane_words:
         _refuse(f"qsgd_decode_clip: {words.numel()} words, {lanes.plane_words} needed")
-    with _on(dev):
-        nt = norm_tensor(norm, dev)
-        if nt.numel() < 1:
-            _refuse("qsgd_decode_clip: empty norm")
-        out = _scalar(g)
-        check(_lib.load().gc_qsgd_decode_clip(_p(words), g.n, _p(nt), int(bits), C.byref(lanes), float(alpha), g._use(),
-                                              code, max_norm, _p(out), _p(_workspace(g)), _stream(dev)),
-              "gc_qsgd_decode_clip")
+    nt = norm_tensor(norm, dev)
+    if nt.numel() < 1:
+        _refuse("qsgd_decode_clip: empty norm")
+    out = g._scalar()
+    ws = g._workspace()
+    _call("gc_qsgd_decode_clip", dev, words.data_ptr(), g.n, nt.data_ptr(), int(bits), C.byref(lanes), float(alpha),
+          g._use(), code, max_norm, out.data_ptr(), ws.data_ptr())
     return out
