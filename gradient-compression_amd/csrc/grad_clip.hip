@@ -10,8 +10,8 @@
 // partials in one fixed order and forms c itself.  So there are no atomics, no
 // tickets and no zeroed state: the result does not depend on the schedule, a
 // captured call owns all that it writes, and two calls on different streams
-// share nothing.  What one block can read in a few microseconds (kOneTiles) is
-// done by one block in one launch.
+// share nothing.  A list that one block can read in a few microseconds
+// (kOneElems) is done by one block in one launch.
 //
 // Sums are held in 64 bits: the square of a float32 is exact to half an ulp
 // there and cannot overflow or vanish, so N is right for any gradients whose
@@ -33,12 +33,19 @@
 
 namespace gc {
 
-constexpr uint32_t kTile = 2048;       // flat elements a wave takes at a time
+constexpr uint32_t kTile = 2048;       // flat elements a wave takes at a time, at most
 constexpr unsigned kNormThreads = 1024;
 constexpr unsigned kNormGrid = 512;    // two blocks a CU: 32 waves, each with 4 KB in flight
 constexpr unsigned kScaleThreads = 256;
-constexpr unsigned kScaleGrid = 2048;
-constexpr uint64_t kOneTiles = 16;     // a tile a wave of one block
+constexpr unsigned kScaleGrid = 16384;
+constexpr unsigned kLaneGrid = 256;
+constexpr unsigned kDecodeGrid = 4096;
+constexpr uint64_t kWaves = 8192;      // resident at once: 256 CUs of 32
+constexpr uint64_t kOneElems = 8192;   // what one block does alone
+constexpr uint32_t kLeastTile = 256;   // a vector a lane
+constexpr uint64_t kFewElems = 1024;   // tensors of fewer elements are small
+constexpr uint64_t kFewEach = 64;      // for each tensor's own norm
+constexpr uint64_t kCacheBytes = 256ull << 20;
 constexpr double kEps = 1e-6;
 
 // workspace: kNormGrid partials (64-bit), kNormGrid maxima (32-bit), then the
@@ -96,7 +103,7 @@ __device__ __forceinline__ void wave_join(A &a)
 }
 
 // the wave's elements x[0 .. cnt), x and cnt the same for all lanes
-template <class T, class F>
+template <class T, bool NT, class F>
 __device__ __forceinline__ void wave_read(Glob<const T> x, uint32_t cnt, F f)
 {
     constexpr uint32_t V = 16 / sizeof(T), step = 64 * V, U = 4;
@@ -106,7 +113,7 @@ __device__ __forceinline__ void wave_read(Glob<const T> x, uint32_t cnt, F f)
         typename VecOf<T, V>::type v[U];
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u)
-            v[u] = ldv<T, V>(x + i + u * step + lane * V);
+            v[u] = ldv<T, V, NT>(x + i + u * step + lane * V);
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
@@ -127,15 +134,36 @@ __device__ __forceinline__ void wave_read(Glob<const T> x, uint32_t cnt, F f)
     }
 }
 
-template <class F>
+template <bool NT, class F>
 __device__ __forceinline__ void wave_read_any(uint32_t type, uint64_t base, uint64_t off, uint32_t cnt, F f)
 {
     if (type == kTF32)
-        wave_read<float>(glob<const float>(base, off), cnt, f);
+        wave_read<float, NT>(glob<const float>(base, off), cnt, f);
     else if (type == kTBF16)
-        wave_read<__bf16>(glob<const __bf16>(base, off), cnt, f);
+        wave_read<__bf16, NT>(glob<const __bf16>(base, off), cnt, f);
     else
-        wave_read<_Float16>(glob<const _Float16>(base, off), cnt, f);
+        wave_read<_Float16, NT>(glob<const _Float16>(base, off), cnt, f);
+}
+
+// f(i, x) for element lo + i of a tile of kLeastTile or fewer elements of
+// tensors s0 .. s1, the lane's own: four lookups, then four loads in flight
+template <class F>
+__device__ __forceinline__ void lane_read(const GradRec *rec, uint32_t s0, uint32_t s1, uint64_t lo, uint64_t hi, F f)
+{
+    constexpr uint32_t U = kLeastTile / 64;
+    float x[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+        const uint64_t e = lo + u * 64 + lane_id();
+        if (e < hi) {
+            const uint32_t s = grad_lane(rec, s0, s1, e);
+            x[u] = ld_any(rec[s].pt, e - rec[s].start);
+        }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+        if (lo + u * 64 + lane_id() < hi)
+            f(u * 64 + lane_id(), x[u]);
 }
 
 // The block's share of the sum of |x|^p and (PEAK) of max |x|, valid in thread 0.
@@ -143,23 +171,59 @@ __device__ __forceinline__ void wave_read_any(uint32_t type, uint64_t base, uint
 // sequence each next piece has the next tile or the next tensor, so a tensor's
 // pieces have consecutive slots of their own.
 template <int P, bool EACH, bool PEAK>
-__device__ __forceinline__ void block_norm(const GradRec *rec, uint32_t count, uint64_t n, double *__restrict__ slots,
+__device__ __forceinline__ void block_norm(const GradRec *rec, uint32_t count, uint64_t n, uint32_t tile, uint64_t cold,
+                                           double *__restrict__ slots,
                                            Acc<P> &all, Acc<kPInf> &top)
 {
     __shared__ double sacc[kNormThreads / 64];
     __shared__ uint32_t smax[kNormThreads / 64];
-    const uint64_t tiles = (n + kTile - 1) / kTile, waves = (uint64_t)gridDim.x * (kNormThreads / 64);
-    for (uint64_t t = (uint64_t)blockIdx.x * (kNormThreads / 64) + wave_id(); t < tiles; t += waves) {
-        const uint64_t lo = t * kTile, hi = min(lo + kTile, n);
-        grad_walk(rec, count, lo, hi,
+    __shared__ double svals[EACH ? kNormThreads / 64 : 1][EACH ? kLeastTile : 1];
+    const uint64_t waves = (uint64_t)gridDim.x * (kNormThreads / 64);
+    for (uint64_t t = (uint64_t)blockIdx.x * (kNormThreads / 64) + wave_id(); t * tile < n; t += waves) {
+        const uint64_t lo = t * tile, hi = min(lo + tile, n);
+        const uint32_t s0 = uni32(grad_find(rec, count, lo));
+        if (tile == kLeastTile && grad_many(rec, count, s0, hi)) {
+            const uint32_t s1 = uni32(grad_find(rec, count, hi - 1));
+            double *v = EACH ? svals[wave_id()] : nullptr;
+            lane_read(rec, s0, s1, lo, hi, [&](uint32_t i, float x) {
+                Acc<P> one;
+                one.add(x);
+                all.join(one);
+                if (PEAK)
+                    top.add(x);
+                if (EACH)
+                    v[i] = one.value();
+            });
+            if (EACH) {  // the pieces' sums, a lane a piece, in the elements' order
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+                for (uint32_t s = s0 + lane_id(); s <= s1; s += 64) {
+                    const uint64_t a = max(rec[s].start, lo), b = min(rec[s + 1].start, hi);
+                    Acc<P> one;
+                    for (uint64_t e = a; e < b; ++e) {
+                        Acc<P> o;
+                        o.set(v[e - lo]);
+                        one.join(o);
+                    }
+                    if (a < b)
+                        slots[t + s] = one.value();
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+            }
+            continue;
+        }
+        grad_walk(rec, s0, lo, hi,
                   [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
                       Acc<P> one;
                       Acc<P> &acc = EACH ? one : all;
-                      wave_read_any(type, base, a - start, (uint32_t)(b - a), [&](float x) {
+                      auto add = [&](float x) {
                           acc.add(x);
                           if (PEAK)
                               top.add(x);
-                      });
+                      };
+                      if (lo < cold)
+                          wave_read_any<true>(type, base, a - start, (uint32_t)(b - a), add);
+                      else
+                          wave_read_any<false>(type, base, a - start, (uint32_t)(b - a), add);
                       if (EACH) {
                           all.join(one);
                           wave_join(one);
@@ -242,12 +306,13 @@ __device__ __forceinline__ void write_norm(int p, double t, double *total, float
 // the norm of tensor s from its slots; the wave's, or (WAVES > 1) the block's:
 // the same number of slots for every wave's share, then the waves in order
 template <int P, unsigned WAVES>
-__device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, const double *slots, float *__restrict__ each)
+__device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, uint32_t tile, const double *slots,
+                                            float *__restrict__ each)
 {
     const uint64_t a = uni64(rec[s].start), b = uni64(rec[s + 1].start);
     double t = 0.0;
     if (a != b) {
-        const uint64_t s0 = a / kTile + s, cnt = (b - 1) / kTile + s + 1 - s0;
+        const uint64_t s0 = a / tile + s, cnt = (b - 1) / tile + s + 1 - s0;
         const uint64_t share = (cnt + WAVES - 1) / WAVES, w0 = WAVES > 1 ? wave_id() * share : 0;
         t = wave_total<P>(slots + s0 + w0, w0 < cnt ? (uint32_t)min(share, cnt - w0) : 0u);
     }
@@ -266,7 +331,8 @@ __device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, cons
 
 // One partial a block; a grid of one block finishes the call itself
 template <int P, bool EACH, bool PEAK, bool LDS>
-__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, double *__restrict__ part,
+__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, uint32_t tile, uint64_t cold,
+                                                               double *__restrict__ part,
                                                                uint32_t *__restrict__ peak, double *slots,
                                                                double *__restrict__ total, float *__restrict__ norm,
                                                                float *__restrict__ each)
@@ -279,7 +345,7 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
     }
     Acc<P> all;
     Acc<kPInf> top;
-    block_norm<P, EACH, PEAK>(rec, g.count, n, slots, all, top);
+    block_norm<P, EACH, PEAK>(rec, g.count, n, tile, cold, slots, all, top);
     if (threadIdx.x == 0) {
         part[blockIdx.x] = all.value();
         if (PEAK)
@@ -289,18 +355,18 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
     }
     if (EACH && gridDim.x == 1)  // behind block_norm's barrier, which the slots' writes are ahead of
         for (uint32_t s = wave_id(); s < g.count; s += kNormThreads / 64)
-            tensor_norm<P, 1>(rec, s, slots, each);
+            tensor_norm<P, 1>(rec, s, tile, slots, each);
 }
 
 // block 0: the total and N; block 1 + s: the norm of tensor s
 template <int P>
-__global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, const double *__restrict__ part, uint32_t parts,
+__global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, uint32_t tile, const double *__restrict__ part, uint32_t parts,
                                                               const double *__restrict__ slots,
                                                               double *__restrict__ total, float *__restrict__ norm,
                                                               float *__restrict__ each)
 {
     if (blockIdx.x > 0) {
-        tensor_norm<P, kNormThreads / 64>(g.rec, blockIdx.x - 1, slots, each);
+        tensor_norm<P, kNormThreads / 64>(g.rec, blockIdx.x - 1, tile, slots, each);
     } else if (wave_id() == 0) {
         const double t = wave_total<P>(part, parts);
         if (lane_id() == 0)
@@ -311,7 +377,7 @@ __global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, const d
 // ---------------------------------------------------------------------------
 // scale
 // ---------------------------------------------------------------------------
-template <class TS, class TD>
+template <class TS, class TD, bool NT>
 __device__ __forceinline__ void wave_scale(Glob<const TS> x, Glob<TD> y, uint32_t cnt, float c)
 {
     constexpr uint32_t V = sizeof(TS) == 2 && sizeof(TD) == 2 ? 8 : 4, step = 64 * V, U = 4;
@@ -321,7 +387,7 @@ __device__ __forceinline__ void wave_scale(Glob<const TS> x, Glob<TD> y, uint32_
         typename VecOf<TS, V>::type v[U];
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u)
-            v[u] = ldv<TS, V>(x + i + u * step + lane * V);
+            v[u] = ldv<TS, V, NT>(x + i + u * step + lane * V);
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             float f[V];
@@ -347,84 +413,112 @@ __device__ __forceinline__ void wave_scale(Glob<const TS> x, Glob<TD> y, uint32_
     }
 }
 
-template <class TS>
+template <class TS, bool NT>
 __device__ __forceinline__ void wave_scale_to(uint32_t td, Glob<const TS> x, uint64_t base, uint64_t off, uint32_t cnt,
                                               float c)
 {
     if (td == kTF32)
-        wave_scale<TS, float>(x, glob<float>(base, off), cnt, c);
+        wave_scale<TS, float, NT>(x, glob<float>(base, off), cnt, c);
     else if (td == kTBF16)
-        wave_scale<TS, __bf16>(x, glob<__bf16>(base, off), cnt, c);
+        wave_scale<TS, __bf16, NT>(x, glob<__bf16>(base, off), cnt, c);
     else
-        wave_scale<TS, _Float16>(x, glob<_Float16>(base, off), cnt, c);
+        wave_scale<TS, _Float16, NT>(x, glob<_Float16>(base, off), cnt, c);
 }
 
-// Tile t of y = RN(x c), from the tensors of src into those of dst (the same
+// The tile from element lo on of y = RN(x c), from the tensors of src into those of dst (the same
 // sizes), or (FLAT) end to end into float32
-template <bool FLAT>
+template <bool FLAT, bool NT>
 __device__ __forceinline__ void scale_tile(const GradRec *rs, const GradRec *rd, uint32_t count, float *flat, uint64_t n,
-                                           uint64_t t, float c)
+                                           uint64_t lo, uint32_t tile, float c)
 {
-    const uint64_t lo = t * kTile, hi = min(lo + kTile, n);
-    grad_walk(rs, count, lo, hi, [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
+    const uint64_t hi = min(lo + tile, n);
+    const uint32_t s0 = uni32(grad_find(rs, count, lo));
+    if (tile == kLeastTile && grad_many(rs, count, s0, hi)) {
+        const uint32_t s1 = uni32(grad_find(rs, count, hi - 1));
+        lane_read(rs, s0, s1, lo, hi, [&](uint32_t i, float x) {
+            const uint64_t e = lo + i;
+            if (FLAT) {
+                flat[e] = x * c;
+            } else {
+                const uint32_t s = grad_lane(rs, s0, s1, e);
+                st_any(rd[s].pt, e - rd[s].start, x * c);
+            }
+        });
+        return;
+    }
+    grad_walk(rs, s0, lo, hi, [&](uint32_t s, uint32_t type, uint64_t base, uint64_t start, uint64_t a, uint64_t b) {
         const uint64_t dpt = FLAT ? (uint64_t)kTF32 << 56 | reinterpret_cast<uint64_t>(flat) : uni64(rd[s].pt);
         const uint64_t off = a - start, doff = FLAT ? a : off;
         const uint32_t td = (uint32_t)(dpt >> 56), cnt = (uint32_t)(b - a);
         const uint64_t dbase = dpt & 0x00ffffffffffffffull;
         if (type == kTF32)
-            wave_scale_to<float>(td, glob<const float>(base, off), dbase, doff, cnt, c);
+            wave_scale_to<float, NT>(td, glob<const float>(base, off), dbase, doff, cnt, c);
         else if (type == kTBF16)
-            wave_scale_to<__bf16>(td, glob<const __bf16>(base, off), dbase, doff, cnt, c);
+            wave_scale_to<__bf16, NT>(td, glob<const __bf16>(base, off), dbase, doff, cnt, c);
         else
-            wave_scale_to<_Float16>(td, glob<const _Float16>(base, off), dbase, doff, cnt, c);
+            wave_scale_to<_Float16, NT>(td, glob<const _Float16>(base, off), dbase, doff, cnt, c);
     });
 }
 
 // The partials' pass has c = 1 in most steps of a training run; in place
 // nothing is left to do then.
 template <bool FLAT, bool LDS>
-__global__ __launch_bounds__(kScaleThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n, int p,
+__global__ __launch_bounds__(kNormThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n, uint32_t tile,
+                                                              uint64_t cold, int p,
                                                               double max_norm, const double *__restrict__ part,
                                                               uint32_t parts, const uint32_t *__restrict__ peaks,
                                                               bool in_place, float *__restrict__ norm,
                                                               float *__restrict__ peak)
 {
-    const double N = root_of(p, wave_total_of(p, part, parts));
-    const float c = clip_coef(N, max_norm);
-    if (blockIdx.x == 0 && wave_id() == 0) {
-        if (FLAT) {
-            // max |RN(x c)| = RN(max |x| c): rounding keeps the order.  A NaN
-            // or infinite x with c = NaN or 0 gives NaN on both sides.
-            Acc<kPInf> top;
-            for (uint32_t i = lane_id(); i < parts; i += 64)
-                top.m = max(top.m, peaks[i]);
-            wave_join(top);
-            if (lane_id() == 0)
-                *peak = __uint_as_float(top.m) * c;
-        }
-        if (norm && lane_id() == 0)
-            *norm = (float)N;
-    }
-    if (in_place && c == 1.0f)
-        return;
     __shared__ GradRec ss[LDS ? kLdsRecs + 1 : 1];
     __shared__ GradRec sd[LDS && !FLAT ? kLdsRecs + 1 : 1];
+    __shared__ float sc;
     const GradRec *rs = LDS ? ss : src.rec, *rd = LDS ? sd : dst.rec;
+    if (wave_id() == 0) {
+        const double N = root_of(p, wave_total_of(p, part, parts));
+        const float c0 = clip_coef(N, max_norm);
+        if (lane_id() == 0)
+            sc = c0;
+        if (blockIdx.x == 0) {
+            if (FLAT) {
+                // max |RN(x c)| = RN(max |x| c): rounding keeps the order.  A NaN
+                // or infinite x with c = NaN or 0 gives NaN on both sides.
+                Acc<kPInf> top;
+                for (uint32_t i = lane_id(); i < parts; i += 64)
+                    top.m = max(top.m, peaks[i]);
+                wave_join(top);
+                if (lane_id() == 0)
+                    *peak = __uint_as_float(top.m) * c0;
+            }
+            if (norm && lane_id() == 0)
+                *norm = (float)N;
+        }
+    }
     if (LDS && n) {
         stage_table(src, ss);
         if (!FLAT)
             stage_table(dst, sd);
-        __syncthreads();
     }
-    const uint64_t tiles = (n + kTile - 1) / kTile, waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
-    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves)
-        scale_tile<FLAT>(rs, rd, src.count, flat, n, tiles - 1 - t, c);
+    __syncthreads();
+    const float c = sc;
+    if (in_place && c == 1.0f)
+        return;
+    const uint32_t per = blockDim.x >> 6;
+    const uint64_t tiles = (n + tile - 1) / tile, waves = (uint64_t)gridDim.x * per;
+    for (uint64_t t = (uint64_t)blockIdx.x * per + wave_id(); t < tiles; t += waves) {
+        const uint64_t lo = t * tile;
+        if (lo < cold)
+            scale_tile<FLAT, true>(rs, rd, src.count, flat, n, lo, tile, c);
+        else
+            scale_tile<FLAT, false>(rs, rd, src.count, flat, n, lo, tile, c);
+    }
 }
 
 // both passes in one block
 template <int P, bool FLAT>
 __global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, GradArg dst, float *flat, uint64_t n,
-                                                                double max_norm, bool in_place, float *__restrict__ norm,
+                                                                uint32_t tile, double max_norm, bool in_place,
+                                                                float *__restrict__ norm,
                                                                 float *__restrict__ peak)
 {
     __shared__ GradRec ss[kLdsRecs + 1];
@@ -438,7 +532,7 @@ __global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, Gra
     }
     Acc<P> all;
     Acc<kPInf> top;
-    block_norm<P, false, FLAT>(ss, src.count, n, nullptr, all, top);
+    block_norm<P, false, FLAT>(ss, src.count, n, tile, 0, nullptr, all, top);
     if (threadIdx.x == 0) {
         const double N = root_of(P, all.value());
         sc = clip_coef(N, max_norm);
@@ -451,9 +545,8 @@ __global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, Gra
     const float c = sc;
     if (in_place && c == 1.0f)
         return;
-    const uint64_t tiles = (n + kTile - 1) / kTile;
-    for (uint64_t t = wave_id(); t < tiles; t += kNormThreads / 64)
-        scale_tile<FLAT>(ss, sd, src.count, flat, n, t, c);
+    for (uint64_t lo = (uint64_t)wave_id() * tile; lo < n; lo += (uint64_t)(kNormThreads / 64) * tile)
+        scale_tile<FLAT, false>(ss, sd, src.count, flat, n, lo, tile, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -469,6 +562,8 @@ struct LaneArg {
     uint32_t w;    // lane width
     uint32_t L;    // lanes a word
     uint32_t qmax; // largest |Q|
+    uint64_t cold; // words the norm reads past the cache
+    uint32_t split; // shares of a tile's planes
 };
 
 // v depends on Q alone, so the norm is |k alpha| times the norm of the
@@ -538,6 +633,13 @@ __device__ __forceinline__ uint32_t quad_sum(const LaneArg &a, uint4 wd, uint64_
     return sum;
 }
 
+__device__ __forceinline__ uint4 ld_nt4u(const uint4 *p)
+{
+    typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+    const u4v v = __builtin_nontemporal_load(reinterpret_cast<const u4v *>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 // the block's share of the norm of the words, valid in thread 0
 template <int P>
 __device__ __forceinline__ uint64_t block_lanes(const LaneArg &a, float k, bool exact)
@@ -560,7 +662,7 @@ __device__ __forceinline__ uint64_t block_lanes(const LaneArg &a, float k, bool 
             uint4 wd[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                wd[u] = words[t + u * stride];
+                wd[u] = 4 * (t + u * stride) < a.cold ? ld_nt4u(words + t + u * stride) : words[t + u * stride];
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 add(wd[u], 4 * (t + u * stride));
@@ -617,9 +719,11 @@ __device__ __forceinline__ void store_quad(uint64_t base, uint64_t start, uint64
             y[i + e - start] = Elem<T>::down(v[e]);
 }
 
-// Tile t: 256 kQuads consecutive words, L ranges of as many flat elements
+// Planes l0 .. l1 - 1 of tile t: of 256 kQuads consecutive words, a range of as
+// many flat elements each
 constexpr int kQuads = 2;
-__device__ __forceinline__ void decode_tile(const LaneArg &a, const GradRec *rd, uint32_t count, uint64_t t, float k, float c)
+__device__ __forceinline__ void decode_tile(const LaneArg &a, const GradRec *rd, uint32_t count, uint64_t t, uint32_t l0,
+                                            uint32_t l1, float k, float c)
 {
     const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u, lane = lane_id();
     const uint64_t j0 = t * (256 * kQuads), j1 = min(j0 + 256 * kQuads, a.M);
@@ -629,11 +733,11 @@ __device__ __forceinline__ void decode_tile(const LaneArg &a, const GradRec *rd,
         const uint64_t j = j0 + 256 * q + 4 * lane;  // M is a multiple of 4: a quad is in or out
         wd[q] = j < j1 ? *reinterpret_cast<const uint4 *>(a.words + j) : make_uint4(0, 0, 0, 0);
     }
-    for (uint32_t l = 0; l < a.L; ++l) {
+    for (uint32_t l = l0; l < l1; ++l) {
         const uint64_t lo = (uint64_t)l * a.M + j0, hi = min((uint64_t)l * a.M + j1, a.n);
         if (lo >= hi)
             break;
-        grad_walk(rd, count, lo, hi, [&](uint32_t, uint32_t type, uint64_t base, uint64_t start, uint64_t pa, uint64_t pb) {
+        grad_walk(rd, uni32(grad_find(rd, count, lo)), lo, hi, [&](uint32_t, uint32_t type, uint64_t base, uint64_t start, uint64_t pa, uint64_t pb) {
 #pragma unroll
             for (int q = 0; q < kQuads; ++q) {
                 if (lo + 256 * q >= pb || lo + 256 * (q + 1) <= pa)
@@ -660,6 +764,13 @@ __device__ __forceinline__ void decode_tile(const LaneArg &a, const GradRec *rd,
 
 __host__ __device__ __forceinline__ uint64_t decode_tiles(uint64_t M) { return (M + 256 * kQuads - 1) / (256 * kQuads); }
 
+// the planes of a tile in a.split shares
+__device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd, uint32_t count, uint64_t u, float k, float c)
+{
+    const uint32_t per = (a.L + a.split - 1) / a.split, l0 = (uint32_t)(u % a.split) * per;
+    decode_tile(a, rd, count, u / a.split, l0, min(l0 + per, a.L), k, c);
+}
+
 template <int P, bool LDS>
 __global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradArg dst, double max_norm,
                                                                const uint64_t *__restrict__ part, uint32_t parts,
@@ -667,22 +778,27 @@ __global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradAr
 {
     const float k = *a.norm / a.s;
     const bool exact = lanes_exact(a, k);
-    uint64_t sum = 0;  // the bits of 0.0 as well
-    for (uint32_t i = lane_id(); i < parts; i += 64)
-        sum = lanes_join<P>(exact, sum, part[i]);
-    const double N = lanes_root<P>(a, k, exact, lanes_wave<P>(exact, sum));
-    const float c = clip_coef(N, max_norm);
-    if (blockIdx.x == 0 && threadIdx.x == 0)
-        *norm = (float)N;
     __shared__ GradRec sd[LDS ? kLdsRecs + 1 : 1];
+    __shared__ float sc;
     const GradRec *rd = LDS ? sd : dst.rec;
-    if (LDS && a.n) {
-        stage_table(dst, sd);
-        __syncthreads();
+    if (wave_id() == 0) {
+        uint64_t sum = 0;  // the bits of 0.0 as well
+        for (uint32_t i = lane_id(); i < parts; i += 64)
+            sum = lanes_join<P>(exact, sum, part[i]);
+        const double N = lanes_root<P>(a, k, exact, lanes_wave<P>(exact, sum));
+        if (lane_id() == 0) {
+            sc = clip_coef(N, max_norm);
+            if (blockIdx.x == 0)
+                *norm = (float)N;
+        }
     }
-    const uint64_t tiles = decode_tiles(a.M), waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
-    for (uint64_t t = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); t < tiles; t += waves)
-        decode_tile(a, rd, dst.count, tiles - 1 - t, k, c);
+    if (LDS && a.n)
+        stage_table(dst, sd);
+    __syncthreads();
+    const float c = sc;
+    const uint64_t units = decode_tiles(a.M) * a.split, waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
+    for (uint64_t u = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); u < units; u += waves)
+        decode_unit(a, rd, dst.count, u, k, c);
 }
 
 // both passes in one block
@@ -703,8 +819,8 @@ __global__ __launch_bounds__(kNormThreads) void k_decode_clip_one(LaneArg a, Gra
         *norm = (float)N;
     }
     __syncthreads();
-    for (uint64_t t = wave_id(), tiles = decode_tiles(a.M); t < tiles; t += kNormThreads / 64)
-        decode_tile(a, sd, dst.count, t, k, sc);
+    for (uint64_t u = wave_id(), units = decode_tiles(a.M) * a.split; u < units; u += kNormThreads / 64)
+        decode_unit(a, sd, dst.count, u, k, sc);
 }
 
 // ---------------------------------------------------------------------------
@@ -817,14 +933,62 @@ static GradArg arg_of(const gc_grads *g)
     return {reinterpret_cast<const GradRec *>(g->rec), (uint32_t)g->count};
 }
 
-static unsigned norm_grid(uint64_t n)
+// the bytes of the gradients
+static uint64_t held_bytes(const gc_grads *g)
 {
-    const uint64_t tiles = (n + kTile - 1) / kTile, per = kNormThreads / 64;
-    return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
+    uint64_t wide = 0;
+    for (uint64_t s = 0; s < g->count; ++s)
+        if (elem_size(g->host_rec[2 * s]) == 4)
+            wide += g->host_rec[2 * s + 3] - g->host_rec[2 * s + 1];
+    return 2 * (g->n + wide);
 }
 
-// whether one block does both passes of a clip of n elements
-static bool one_block(uint64_t n, uint64_t count) { return n <= kOneTiles * kTile && count <= kLdsRecs; }
+// The elements of a wave's tile: `most`, or as few as spread a short list over
+// the chip (over the waves of the one block that does all of it); the least for
+// tensors that are small on the whole, which a lane at a time takes.
+static uint32_t tile_of(uint64_t n, uint64_t count, uint32_t most, uint64_t few = kFewElems)
+{
+    if (n < few * count)
+        return kLeastTile;
+    const uint64_t want = n <= kOneElems ? kNormThreads / 64 : 2 * kWaves;
+    uint32_t tile = most;
+    while (tile > kLeastTile && n <= (uint64_t)(tile / 2) * want)
+        tile /= 2;
+    return tile;
+}
+
+// Whether one block does all of a call: a second launch costs 2 us, a tensor
+// about what eight elements do.  Clipping 5000 elements of 3 / 60 / 500 tensors
+// takes 6.3 / 11.6 / 18.3 us in one block and 8.3 / 11.1 / 13.4 us in two
+// launches, 20000 of 3 / 60 tensors 8.8 / 19.2 and 9.5 / 11.1 us.
+static bool one_block(uint64_t n, uint64_t count) { return n + 8 * count <= kOneElems; }
+
+// The norm's tile: up to 8 KB of gradients.  Each tensor's own norm takes a
+// lane a tensor there, one element after the other, so only the smallest.
+static uint32_t norm_tile(const gc_grads *g, bool each = false)
+{
+    return tile_of(g->n, g->count, held_bytes(g) < 3 * g->n ? 2 * kTile : kTile, each ? kFewEach : kFewElems);
+}
+
+static unsigned norm_grid(uint64_t n, uint64_t count, uint32_t tile)
+{
+    const uint64_t tiles = (n + tile - 1) / tile, per = kNormThreads / 64;
+    return one_block(n, count) ? 1u : (unsigned)std::min<uint64_t>((tiles + per - 1) / per, kNormGrid);
+}
+
+// of `of` elements or words that take `bytes`, those ahead of the last kCacheBytes
+static uint64_t cold_part(uint64_t of, uint64_t bytes)
+{
+    return bytes <= kCacheBytes ? 0 : (uint64_t)((double)(bytes - kCacheBytes) / (double)bytes * (double)of);
+}
+static uint64_t cold_elems(const gc_grads *g) { return cold_part(g->n, held_bytes(g)); }
+
+// shares of the planes for which `tiles` tiles of words keep the chip's waves busy
+static uint32_t split_of(uint64_t tiles, uint32_t L)
+{
+    const uint64_t want = kWaves / 2;
+    return tiles >= want ? 1u : (uint32_t)std::min<uint64_t>(L, (want + tiles - 1) / std::max<uint64_t>(tiles, 1));
+}
 
 // f(p as a constant)
 template <class F>
@@ -839,29 +1003,37 @@ static void with_p(uint32_t p, F f)
 }
 
 template <bool EACH, bool PEAK>
-static void launch_norm(const gc_grads *g, uint32_t p, void *ws, double *total, float *norm, float *each, hipStream_t st)
+static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, double *total, float *norm, float *each,
+                        hipStream_t st)
 {
     const GradArg a = arg_of(g);
-    const dim3 grid(norm_grid(g->n)), block(kNormThreads);
+    const uint32_t tile = norm_tile(g, EACH);
+    const dim3 grid(norm_grid(g->n, g->count, tile)), block(kNormThreads);
     char *w = static_cast<char *>(ws);
     double *part = reinterpret_cast<double *>(w);
     uint32_t *peak = reinterpret_cast<uint32_t *>(w + kWsPeak);
     double *slots = reinterpret_cast<double *>(w + kWsSlots);
     with_p(p, [&](auto P) {
         if (g->count <= kLdsRecs)
-            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, part, peak, slots, total,
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, tile, cold, part, peak, slots,
+                               total,
                                norm, each);
         else
-            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, part, peak, slots, total,
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, tile, cold, part, peak, slots,
+                               total,
                                norm, each);
     });
 }
 
-static unsigned scale_grid(uint64_t tiles)
+static unsigned grid_of(uint64_t tiles, unsigned threads, unsigned most)
 {
-    const uint64_t per = kScaleThreads / 64;
-    return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kScaleGrid);
+    const uint64_t per = threads / 64;
+    return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), most);
 }
+
+// threads a block of the scale: large blocks, and so fewer first steps (the
+// partials, the table), where all tiles are under way at once
+static unsigned scale_threads(uint64_t tiles) { return tiles <= kWaves ? kNormThreads : kScaleThreads; }
 
 }  // namespace gc
 
@@ -938,7 +1110,7 @@ int gc_grads_fill(const gc_grads *grads, uint64_t *rec, gc_stream_t stream)
 
 size_t gc_grad_workspace_size(uint64_t n, uint64_t count, int each)
 {
-    return kWsSlots + (each ? ((n + kTile - 1) / kTile + count) * sizeof(double) : 0);
+    return kWsSlots + (each ? (n / tile_of(n, count, kTile, kFewEach) + 1 + count) * sizeof(double) : 0);
 }
 
 int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, float *each, void *workspace,
@@ -951,15 +1123,16 @@ int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, 
     GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
     hipStream_t st = as_stream(stream);
     if (each)
-        launch_norm<true, false>(grads, p, workspace, total, norm, each, st);
+        launch_norm<true, false>(grads, p, ~0ull, workspace, total, norm, each, st);
     else
-        launch_norm<false, false>(grads, p, workspace, total, norm, each, st);
-    const unsigned parts = norm_grid(grads->n);
+        launch_norm<false, false>(grads, p, ~0ull, workspace, total, norm, each, st);
+    const uint32_t tile = norm_tile(grads, each != nullptr);
+    const unsigned parts = norm_grid(grads->n, grads->count, tile);
     if (parts > 1) {
         const char *w = static_cast<const char *>(workspace);
         const dim3 grid(1 + (each ? (unsigned)grads->count : 0u));
         with_p(p, [&](auto P) {
-            hipLaunchKernelGGL(k_grad_finish<P()>, grid, dim3(kNormThreads), 0, st, arg_of(grads),
+            hipLaunchKernelGGL(k_grad_finish<P()>, grid, dim3(kNormThreads), 0, st, arg_of(grads), tile,
                                reinterpret_cast<const double *>(w), parts, reinterpret_cast<const double *>(w + kWsSlots),
                                total, norm, each);
         });
@@ -975,7 +1148,7 @@ int gc_grad_norm_root(const double *total, uint32_t p, float *norm, gc_stream_t 
         return rc;
     GC_REQUIRE(total && norm, "%s: null pointer", what);
     with_p(p, [&](auto P) {
-        hipLaunchKernelGGL(k_grad_finish<P()>, dim3(1), dim3(64), 0, as_stream(stream), GradArg{nullptr, 0}, total, 1u,
+        hipLaunchKernelGGL(k_grad_finish<P()>, dim3(1), dim3(64), 0, as_stream(stream), GradArg{nullptr, 0}, kTile, total, 1u,
                            nullptr, nullptr, norm, nullptr);
     });
     return launch_status(what);
@@ -1001,24 +1174,26 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
     GC_REQUIRE(total || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0),
                "%s: null or misaligned workspace", what);
     hipStream_t st = as_stream(stream);
-    if (!total && one_block(src->n, src->count)) {
+    if (!total && src->count <= kLdsRecs && one_block(src->n, src->count)) {
         with_p(p, [&](auto P) {
             hipLaunchKernelGGL((k_grad_clip_one<P(), false>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), arg_of(dst),
-                               nullptr, src->n, max_norm, same, norm, nullptr);
+                               nullptr, src->n, tile_of(src->n, src->count, kTile), max_norm, same, norm, nullptr);
         });
         return launch_status(what);
     }
     if (!total)
-        launch_norm<false, false>(src, p, workspace, nullptr, nullptr, nullptr, st);
+        launch_norm<false, false>(src, p, cold_elems(src), workspace, nullptr, nullptr, nullptr, st);
     const double *part = total ? total : static_cast<const double *>(workspace);
-    const unsigned parts = total ? 1u : norm_grid(src->n);
-    const unsigned grid = scale_grid((src->n + kTile - 1) / kTile);
+    const unsigned parts = total ? 1u : norm_grid(src->n, src->count, norm_tile(src));
+    const uint32_t tile = tile_of(src->n, src->count, kTile);
+    const uint64_t tiles = (src->n + tile - 1) / tile;
+    const unsigned threads = scale_threads(tiles), grid = grid_of(tiles, threads, kScaleGrid);
     const GradArg a = arg_of(src), b = arg_of(dst);
     if (src->count <= kLdsRecs)
-        hipLaunchKernelGGL((k_grad_scale<false, true>), dim3(grid), dim3(kScaleThreads), 0, st, a, b, nullptr, src->n,
+        hipLaunchKernelGGL((k_grad_scale<false, true>), dim3(grid), dim3(threads), 0, st, a, b, nullptr, src->n, tile, cold_elems(src),
                            (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
     else
-        hipLaunchKernelGGL((k_grad_scale<false, false>), dim3(grid), dim3(kScaleThreads), 0, st, a, b, nullptr, src->n,
+        hipLaunchKernelGGL((k_grad_scale<false, false>), dim3(grid), dim3(threads), 0, st, a, b, nullptr, src->n, tile, cold_elems(src),
                            (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
     return launch_status(what);
 }
@@ -1040,24 +1215,26 @@ int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double ma
                    (unsigned long long)s);
     }
     hipStream_t st = as_stream(stream);
-    if (one_block(src->n, src->count)) {
+    if (src->count <= kLdsRecs && one_block(src->n, src->count)) {
         with_p(p, [&](auto P) {
             hipLaunchKernelGGL((k_grad_clip_one<P(), true>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), GradArg{}, flat,
-                               src->n, max_norm, false, norm, peak);
+                               src->n, tile_of(src->n, src->count, kTile), max_norm, false, norm, peak);
         });
         return launch_status(what);
     }
-    launch_norm<false, true>(src, p, workspace, nullptr, nullptr, nullptr, st);
+    launch_norm<false, true>(src, p, cold_elems(src), workspace, nullptr, nullptr, nullptr, st);
     const char *w = static_cast<const char *>(workspace);
-    const unsigned grid = scale_grid((src->n + kTile - 1) / kTile), parts = norm_grid(src->n);
+    const uint32_t tile = tile_of(src->n, src->count, kTile);
+    const uint64_t tiles = (src->n + tile - 1) / tile;
+    const unsigned threads = scale_threads(tiles), grid = grid_of(tiles, threads, kScaleGrid), parts = norm_grid(src->n, src->count, norm_tile(src));
     const GradArg a = arg_of(src);
     const double *part = reinterpret_cast<const double *>(w);
     const uint32_t *peaks = reinterpret_cast<const uint32_t *>(w + kWsPeak);
     if (src->count <= kLdsRecs)
-        hipLaunchKernelGGL((k_grad_scale<true, true>), dim3(grid), dim3(kScaleThreads), 0, st, a, GradArg{}, flat, src->n,
+        hipLaunchKernelGGL((k_grad_scale<true, true>), dim3(grid), dim3(threads), 0, st, a, GradArg{}, flat, src->n, tile, cold_elems(src),
                            (int)p, max_norm, part, parts, peaks, false, norm, peak);
     else
-        hipLaunchKernelGGL((k_grad_scale<true, false>), dim3(grid), dim3(kScaleThreads), 0, st, a, GradArg{}, flat, src->n,
+        hipLaunchKernelGGL((k_grad_scale<true, false>), dim3(grid), dim3(threads), 0, st, a, GradArg{}, flat, src->n, tile, cold_elems(src),
                            (int)p, max_norm, part, parts, peaks, false, norm, peak);
     return launch_status(what);
 }
@@ -1084,15 +1261,15 @@ int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, ui
                "%s: output tensor %llu shares memory with the words or the norm", what, (unsigned long long)at);
     hipStream_t st = as_stream(stream);
     const LaneArg a{words, n, lanes->plane_words, norm, (float)s, alpha, (int32_t)(lanes->world * s), lanes->bits,
-                    lanes->per_word, lanes->world * s};
+                    lanes->per_word, lanes->world * s, cold_part(lanes->plane_words, 4 * lanes->plane_words),
+                    split_of(decode_tiles(lanes->plane_words), lanes->per_word)};
     const uint64_t quads = lanes->plane_words >> 2;
-    const unsigned parts =
-        (unsigned)std::min<uint64_t>(std::max<uint64_t>((quads + kNormThreads - 1) / kNormThreads, 1), kNormGrid);
+    const unsigned parts = grid_of((quads + 63) / 64, kNormThreads, kLaneGrid);
     uint64_t *part = static_cast<uint64_t *>(workspace);
     const GradArg d = arg_of(dst);
-    const dim3 grid(scale_grid(decode_tiles(lanes->plane_words)));
+    const dim3 grid(grid_of(decode_tiles(lanes->plane_words) * a.split, kScaleThreads, kDecodeGrid));
     with_p(p, [&](auto P) {
-        if (one_block(n, dst->count)) {
+        if (dst->count <= kLdsRecs && n <= kOneElems) {
             hipLaunchKernelGGL(k_decode_clip_one<P()>, dim3(1), dim3(kNormThreads), 0, st, a, d, max_norm, total_norm);
             return;
         }

@@ -67,11 +67,11 @@ __device__ __forceinline__ uint32_t grad_find(const GradRec *rec, uint32_t count
 }
 
 // f(s, type, base, start, a, b) for every piece [a, b) of the non-empty flat
-// range [lo, hi), hi <= n; s the tensor, base its address, start its first element
+// range [lo, hi), hi <= n, whose first element is in tensor s; s the piece's
+// tensor, base its address, start its first element
 template <class F>
-__device__ __forceinline__ void grad_walk(const GradRec *rec, uint32_t count, uint64_t lo, uint64_t hi, F f)
+__device__ __forceinline__ void grad_walk(const GradRec *rec, uint32_t s, uint64_t lo, uint64_t hi, F f)
 {
-    uint32_t s = uni32(grad_find(rec, count, lo));
     uint64_t a = lo;
     for (;;) {
         const uint64_t pt = uni64(rec[s].pt), start = uni64(rec[s].start), end = uni64(rec[s + 1].start);
@@ -83,6 +83,27 @@ __device__ __forceinline__ void grad_walk(const GradRec *rec, uint32_t count, ui
         a = end;
         ++s;
     }
+}
+
+// Whether [lo, hi), which begins in tensor s, may span more than three tensors.
+// A walk waits for the memory once a piece: a range of many takes its elements
+// lane by lane instead, each lane with the tensors of its own (grad_lane).
+__device__ __forceinline__ bool grad_many(const GradRec *rec, uint32_t count, uint32_t s, uint64_t hi)
+{
+    return uni64(rec[min(s + 3, count)].start) < hi;
+}
+
+// the lane's tensor of element e, known to be in s .. last
+__device__ __forceinline__ uint32_t grad_lane(const GradRec *rec, uint32_t s, uint32_t last, uint64_t e)
+{
+    while (s < last) {
+        const uint32_t mid = (s + last + 1) >> 1;
+        if (rec[mid].start <= e)
+            s = mid;
+        else
+            last = mid - 1;
+    }
+    return s;
 }
 
 // ---------------------------------------------------------------------------
@@ -124,10 +145,11 @@ __device__ __forceinline__ Glob<T> glob(uint64_t base, uint64_t off)
     return reinterpret_cast<Glob<T>>(base) + off;
 }
 
-template <class T, int V>
+template <class T, int V, bool NT = false>
 __device__ __forceinline__ typename VecOf<T, V>::type ldv(Glob<const T> p)
 {
-    return *reinterpret_cast<Glob<const typename VecOf<T, V>::type>>(p);
+    const auto v = reinterpret_cast<Glob<const typename VecOf<T, V>::type>>(p);
+    return NT ? __builtin_nontemporal_load(v) : *v;
 }
 
 template <class T, int V>
@@ -138,6 +160,28 @@ __device__ __forceinline__ void stv(Glob<T> p, const float (&v)[V])
     for (int k = 0; k < V; ++k)
         o[k] = Elem<T>::down(v[k]);
     __builtin_nontemporal_store(o, reinterpret_cast<Glob<typename VecOf<T, V>::type>>(p));
+}
+
+// one element of a lane's own tensor
+__device__ __forceinline__ float ld_any(uint64_t pt, uint64_t off)
+{
+    const uint32_t type = (uint32_t)(pt >> 56);
+    const uint64_t base = pt & 0x00ffffffffffffffull;
+    if (type == kTF32)
+        return *glob<const float>(base, off);
+    const uint16_t h = *glob<const uint16_t>(base, off);
+    return type == kTBF16 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+}
+__device__ __forceinline__ void st_any(uint64_t pt, uint64_t off, float v)
+{
+    const uint32_t type = (uint32_t)(pt >> 56);
+    const uint64_t base = pt & 0x00ffffffffffffffull;
+    if (type == kTF32)
+        *glob<float>(base, off) = v;
+    else if (type == kTBF16)
+        *glob<__bf16>(base, off) = Elem<__bf16>::down(v);
+    else
+        *glob<_Float16>(base, off) = Elem<_Float16>::down(v);
 }
 
 }  // namespace gc
