@@ -7,6 +7,7 @@ is visible, every codec call raises GCodecError — there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 import threading
 
@@ -205,6 +206,24 @@ def load():
                     fn.argtypes = args
                 _lib = lib
     return _lib
+
+
+_tensor_list = None
+
+
+def tensor_list():
+    """The CPython module that reads lists of tensors (csrc/tensor_list.cpp)."""
+    global _tensor_list
+    if _tensor_list is None:
+        path = os.path.join(PKG_ROOT, "lib", "_tensor_list.so")
+        if not os.path.exists(path):
+            raise GCodecError(GC_ENODEV, f"_tensor_list.so not built ({path}); run "
+                              "`python -c 'import __graft_entry__ as g; g.build()'`")
+        spec = importlib.util.spec_from_file_location("_tensor_list", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _tensor_list = module
+    return _tensor_list
 
 
 def last_error() -> str:

@@ -29,17 +29,14 @@ from __future__ import annotations
 import ctypes as C
 import math
 import numbers
-import operator
 
-import numpy as np
 import torch
 import torch.distributed as dist
 
 from . import _lib
 from .codec import _dev, _raw_stream, norm_tensor, qsgd_layout
 
-_TYPE = {torch.float32: _lib.GC_F32, torch.float16: _lib.GC_F16, torch.bfloat16: _lib.GC_BF16}
-_dtype_of, _grad_of = operator.attrgetter("dtype"), operator.attrgetter("grad")
+_DEVICES = {}  # index -> torch.device
 
 
 def _refuse(msg: str):
@@ -76,16 +73,10 @@ def _call(name: str, device, *args):
         raise _lib.GCodecError(rc, f"{name}: {_lib.last_error()}")
 
 
-def _dense(t: torch.Tensor) -> bool:
-    """Whether the tensor fills its range of memory once, in any order of its dimensions."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, sz) for sz, st in zip(t.shape, t.stride()) if sz != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
+def _on_gpu(t: torch.Tensor) -> torch.device:
+    """t's device, always with its index."""
+    dev = _dev(t)
+    return dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
 class Grads:
@@ -102,64 +93,52 @@ class Grads:
 
     def __init__(self, tensors):
         tensors = list(tensors)
-        self._build(tensors)
+        if not self._build(tensors):
+            _refuse("Grads: empty tensor list")
         if torch.cuda.is_current_stream_capturing():
             _refuse("Grads: made under graph capture; make the table before it")
-        rec = torch.from_numpy(self._host.view(np.int64))
+        rec = torch.frombuffer(bytearray(self._host), dtype=torch.int64)
         self._rec = rec.to(self.device)  # complete when this returns, whatever stream reads it
         self._home = _raw_stream(self.device.index)
         self.struct.rec = self._rec.data_ptr()
         self._keep = [t.untyped_storage() for t in tensors]
 
     @classmethod
-    def _of_call(cls, tensors, ordered=True):
-        """The table of a list for the length of one call, filled on the current stream."""
+    def _of_call(cls, tensors, of_grads=False, ordered=True):
+        """The table of a list (of_grads: of the list's gradients; None if there are none) for the length of
+        one call, filled on the current stream."""
         self = cls.__new__(cls)
-        self._build(tensors, ordered)
-        self._rec = torch.empty(self._host.size, dtype=torch.int64, device=self.device)
+        if not self._build(tensors, of_grads, ordered):
+            return None
+        self._rec = torch.empty(len(self._host) // 8, dtype=torch.int64, device=self.device)
         self._home = None
-        self.struct.rec = self._rec.data_ptr()
-        _call("gc_grads_fill", self.device, self._ref, self.struct.rec)
+        self.struct.rec = rec = self._rec.data_ptr()
+        _call("gc_grads_fill", self.device, self._ref, rec)
         return self
 
-    def _build(self, tensors, ordered=True):
+    def _build(self, tensors, of_grads=False, ordered=True) -> bool:
         """ordered: element i of a tensor is its i-th in row-major order (else any dense order does)"""
-        if not tensors:
-            _refuse("Grads: empty tensor list")
-        try:
-            devices = set(map(torch.Tensor.get_device, tensors))
-            dtypes = set(map(_dtype_of, tensors))
-            contiguous = all(map(torch.Tensor.is_contiguous, tensors))
-        except (TypeError, RuntimeError):  # not a tensor; a sparse one has no strides
-            _refuse("Grads: not a list of dense tensors")
-        self.device = _dev(tensors[0])
-        if len(devices) != 1:
-            _refuse("Grads: the tensors are on different devices")
-        if not dtypes <= _TYPE.keys():
-            _refuse(f"Grads: {(dtypes - _TYPE.keys()).pop()} is not float32, float16 or bfloat16")
-        if not contiguous:
-            bad = [i for i, t in enumerate(tensors) if not (t.is_contiguous() if ordered else _dense(t))]
-            if bad:
-                t = tensors[bad[0]]
-                _refuse(f"Grads: tensor {bad[0]} is not {'contiguous' if ordered else 'dense'} (shape {tuple(t.shape)}, "
-                        f"strides {t.stride()})")
         lib = _lib.load()
-        self.count = count = len(tensors)
-        sizes = (C.c_uint64 * count)(*map(torch.Tensor.numel, tensors))
-        ptrs = (C.c_uint64 * count)(*map(torch.Tensor.data_ptr, tensors))
-        if len(dtypes) == 1:
-            kinds = (C.c_uint32 * count)(*(_TYPE[dtypes.pop()],) * count)
-        else:
-            kinds = (C.c_uint32 * count)(*map(_TYPE.__getitem__, map(_dtype_of, tensors)))
-        self._host = np.empty(2 * (count + 1), dtype=np.uint64)
-        self._order = np.empty(count, dtype=np.uint32)
         self.struct = _lib.gc_grads()
         self._ref = C.byref(self.struct)
-        rc = lib.gc_grads_plan(sizes, ptrs, kinds, count, self._host.ctypes.data, self._order.ctypes.data, self._ref)
-        if rc < 0:
-            raise _lib.GCodecError(rc, f"gc_grads_plan: {_lib.last_error()}")
-        self.n = int(self.struct.n)
-        self._ws = lib.gc_grad_workspace_size(self.n, count, 0)
+        try:
+            got = _lib.tensor_list().gather(tensors, of_grads, ordered, C.cast(lib.gc_grads_plan, C.c_void_p).value,
+                                            C.addressof(self.struct))
+        except LookupError as e:
+            raise _lib.GCodecError(_lib.GC_ENODEV, f"gcodec runs on the GPU only: {e}; there is no CPU fallback") from None
+        except ValueError as e:
+            _refuse(f"Grads: {e}")
+        except RuntimeError as e:
+            _refuse(f"Grads: {e}: {_lib.last_error()}")
+        if got is None:
+            return False
+        index, self._host, self._order = got  # the struct points into these
+        _lib.require_device(index)
+        self.device = _DEVICES.get(index)
+        if self.device is None:
+            self.device = _DEVICES[index] = torch.device("cuda", index)
+        self.count, self.n = self.struct.count, self.struct.n
+        return True
 
     def _use(self):
         """The table for a launch; the allocator is told of a stream other than the one the table was made on."""
@@ -169,7 +148,7 @@ class Grads:
         return self._ref
 
     def _workspace(self, each: bool = False) -> torch.Tensor:
-        size = _lib.load().gc_grad_workspace_size(self.n, self.count, 1) if each else self._ws
+        size = _lib.load().gc_grad_workspace_size(self.n, self.count, each)
         return torch.empty(size, dtype=torch.uint8, device=self.device)
 
     def _scalar(self, dtype=torch.float32) -> torch.Tensor:
@@ -181,7 +160,10 @@ def _table(grads, ordered=True) -> Grads:
         return grads
     if isinstance(grads, torch.Tensor):
         grads = [grads]
-    return Grads._of_call(list(grads), ordered)
+    g = Grads._of_call(grads if isinstance(grads, (list, tuple)) else list(grads), False, ordered)
+    if g is None:
+        _refuse("Grads: empty tensor list")
+    return g
 
 
 def _sum_ranks(total: torch.Tensor, code: int, group) -> torch.Tensor:
@@ -264,8 +246,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     torch.nn.utils.clip_grad_norm_, with the norm held in 64 bits."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [g for g in map(_grad_of, parameters) if g is not None]
-    if not grads:
+    src = Grads._of_call(parameters, True, False)
+    if src is None:
         dev = parameters[0].device if parameters else None
         norm = torch.zeros((), dtype=torch.float64, device=dev)
         if group is not None:  # the other ranks wait for this one's share
@@ -276,11 +258,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         if error_if_nonfinite:
             _finite(norm, "clip_grad_norm_")
         return norm
-    src = _table(grads, ordered=False)
     norm = _clip(src, src, max_norm, code, error_if_nonfinite, group, "clip_grad_norm_")
-    if any(map(torch.Tensor.is_inference, grads)):  # these have no version
-        grads = [g for g in grads if not g.is_inference()]
-    torch.autograd.graph.increment_version(grads)
+    _lib.tensor_list().written(parameters, True)
     return norm
 
 
@@ -308,7 +287,7 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     the gradient tensors, clipped by the norm of all of them; -> that norm
     before clipping.  The unclipped gradients are never stored."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
-    dev = _dev(words)
+    dev = _on_gpu(words)
     g = _table(grads)
     if dev != g.device:
         _refuse(f"qsgd_decode_clip: words on {dev}, gradients on {g.device}")

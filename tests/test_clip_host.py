@@ -156,16 +156,6 @@ def test_python_refusals():
     assert clip.clip_grad_norm_([], 1.0).item() == 0.0
 
 
-@pytest.mark.parametrize("shape,perm,dense", [
-    ((4, 5, 6), (2, 0, 1), True), ((4, 1, 6), (1, 2, 0), True), ((3, 4), (1, 0), True)])
-def test_dense_orders(shape, perm, dense):
-    t = torch.zeros(shape).permute(perm)
-    assert clip._dense(t) == dense
-    assert clip._dense(torch.zeros(2, 3, 4, 5).to(memory_format=torch.channels_last))
-    assert not clip._dense(torch.zeros(4, 6)[:, :3])
-    assert not clip._dense(torch.zeros(4, 1).expand(4, 5))
-
-
 WORKER = r"""
 import math, sys
 sys.path[:0] = [sys.argv[3], sys.argv[4]]
