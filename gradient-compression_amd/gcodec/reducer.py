@@ -17,6 +17,15 @@ all-reduces int8/int32 q (which overflows int8 once W*(2^b-1) > 127); the
 packed lanes are sized for W so the SUM never carries (SURVEY §7 hard part 4).
 Outputs equal the reference's (torch-mode RNG) for every W where the
 reference does not overflow.
+
+Clipping by the global 2-norm (gcodec.clip), which a trainer puts around the
+reducer, can be part of the step: local_max_norm= clips this rank's gradient as
+it is flattened, ahead of the codec (each rank by its own norm; a limit of
+m / sqrt(W) keeps independent gradients' sum at m); max_grad_norm= clips the
+averaged gradient as it is written to grad_out.  The norms before clipping are
+left in `local_grad_norm` and `grad_norm` (float32 scalars on the device).
+The averaged gradient is the same on every rank, and so is its clipping, but
+for the GlobalRandK reducers: their unselected coordinates are each rank's own.
 """
 from __future__ import annotations
 
@@ -28,6 +37,7 @@ import numpy as np
 import torch
 import torch.distributed as dist
 
+from . import clip as _hip_clip
 from . import codec as _hip_codec
 from . import compressors as C
 from .rng import default_generator
@@ -53,7 +63,8 @@ class Reducer:
 
     SEG_CACHE = 8  # gc_segments tables kept (grad_in + grad_out lists of a few recent steps)
 
-    def __init__(self, device, timer=None, codec=None, generator=None, group=None, fused=True, topology=None):
+    def __init__(self, device, timer=None, codec=None, generator=None, group=None, fused=True, topology=None,
+                 max_grad_norm=None, local_max_norm=None):
         if dist.is_available() and dist.is_initialized():
             self.n_workers = dist.get_world_size(group)
             self.rank = dist.get_rank(group)
@@ -69,6 +80,14 @@ class Reducer:
         if topology is not None and group is not None:
             raise ValueError("topology spans the default process group; pass one or the other")
         self._fused = fused
+        self._max_grad_norm = max_grad_norm
+        self._local_max_norm = local_max_norm
+        self.grad_norm = None        # norm of the last averaged gradient before max_grad_norm
+        self.local_grad_norm = None  # norm of this rank's last gradient before local_max_norm
+        # a codec other than the HIP one brings its own clip operators, or has none
+        self._clip = _hip_clip if self._codec is _hip_codec else getattr(self._codec, "clip", None)
+        if self._clip is None and not (max_grad_norm is None and local_max_norm is None):
+            raise ValueError("max_grad_norm / local_max_norm: this codec has no clip operators")
         self._seg_cache = collections.OrderedDict()  # LRU of gc_segments tables by tensor-list key
 
     def reduce(self, grad_in, grad_out):
@@ -140,6 +159,11 @@ class Reducer:
         """reducer.py:512-516: TensorBuffer(grad_in) (+ the local max-norm).
         Fused: one pass over the tensors writes the flat bucket and the norm.
         -> (flat TensorBuffer, local norm or None)"""
+        if self._local_max_norm is not None:
+            grad_in = list(grad_in)
+            with self._timer("reduce.flat_pack"):
+                buf, norm, self.local_grad_norm = self._clip.flatten_clip(grad_in, self._local_max_norm)
+            return TensorBuffer.of_flat(grad_in, buf), norm
         segs = self._segments(grad_in)
         if segs is None:
             with self._timer("reduce.flat_pack"):
@@ -148,6 +172,13 @@ class Reducer:
         with self._timer("reduce.flat_pack"):
             buf, norm = self._codec.segments_flatten_absmax(segs)
         return TensorBuffer.of_flat(grad_in, buf), norm
+
+    def _clip_out(self, grad_out):
+        """max_grad_norm on a written grad_out."""
+        if self._max_grad_norm is not None:
+            with self._timer("reduce.clip", verbosity=2):
+                outs = list(grad_out)
+                self.grad_norm = self._clip.clip_grads(outs, outs, self._max_grad_norm)
 
     def _max_norm(self, flat, local=None, idx=None):
         with self._timer("reduce.norm", verbosity=2):
@@ -212,6 +243,11 @@ class QSGDMaxNormReducer(Reducer):
         with self._timer("reduce.reduce.vector", verbosity=2):
             self._all_reduce(words)
         bits = self.n_bits(norm) + self.n_bits(words)
+        if self._max_grad_norm is not None:  # the norm is taken from the words: decode + 1/W + clipping in one write
+            with self._timer("reduce.decompress", verbosity=2):
+                self.grad_norm = self._clip.qsgd_decode_clip(words, norm, self._quantization_level, list(grad_out),
+                                                             self._max_grad_norm, world=W, alpha=1.0 / W)
+            return bits
         out_segs = self._segments(grad_out)
         with self._timer("reduce.decompress", verbosity=2):
             if out_segs is not None:  # decode + 1/W straight into grad_out (setgrad fused)
@@ -304,8 +340,8 @@ class GlobalRandKMaxNormReducer(Reducer):
         """(in, out) tables when both lists are fused-addressable with equal
         tensor sizes and the subset fits the gather kernel, else None."""
         codec = self._codec
-        if not hasattr(codec, "randk_gather_absmax_segments"):
-            return None
+        if not hasattr(codec, "randk_gather_absmax_segments") or self._local_max_norm is not None:
+            return None  # (a local clipping writes the flat bucket)
         in_segs = self._segments(grad_in)
         out_segs = self._segments(grad_out) if in_segs is not None else None
         if out_segs is None or in_segs.key[1] != out_segs.key[1] or min(self._K, in_segs.n) > codec.RANDK_GATHER_MAX:
@@ -317,7 +353,9 @@ class GlobalRandKMaxNormReducer(Reducer):
         comp = self._randk_compressor()
         pair = self._segment_pair(grad_in, grad_out)
         if pair is not None:
-            return self._reduce_segments(comp, *pair)
+            bits = self._reduce_segments(comp, *pair)
+            self._clip_out(grad_out)
+            return bits
         flat, _ = self._flat_pack(grad_in)
         n = flat.buffer.numel()
         idx = self._next_indices(n, flat.buffer.device)
@@ -345,6 +383,7 @@ class GlobalRandKMaxNormReducer(Reducer):
             comp.decode(norm, words, k, world=W, alpha=1.0, idx=idx, out=flat.buffer)
         with self._timer("reduce.setgrad", verbosity=2):
             self._setgrad_scaled(flat, grad_out, 1.0 / W)
+        self._clip_out(grad_out)
         return bits
 
 
@@ -403,6 +442,7 @@ class QSGDMaxNormTwoScaleReducer(Reducer):
         with self._timer("reduce.setgrad", verbosity=2):
             if out_segs is None:
                 self._setgrad(flat, grad_out)
+        self._clip_out(grad_out)
         return bits
 
 
@@ -454,7 +494,9 @@ class GlobalRandKMaxNormTwoScaleReducer(QSGDMaxNormTwoScaleReducer):
         comp = self._make()
         pair = self._segment_pair(grad_in, grad_out)
         if pair is not None and hasattr(comp, "decode_scatter_segments"):
-            return self._reduce_segments(comp, *pair)
+            bits = self._reduce_segments(comp, *pair)
+            self._clip_out(grad_out)
+            return bits
         flat, _ = self._flat_pack(grad_in)
         n = flat.buffer.numel()
         idx = self._next_indices(n, flat.buffer.device)
@@ -464,6 +506,7 @@ class GlobalRandKMaxNormTwoScaleReducer(QSGDMaxNormTwoScaleReducer):
             comp.decode(norm, words, mask, k, world=W, alpha=1.0, idx=idx, out=flat.buffer)
         with self._timer("reduce.setgrad", verbosity=2):
             self._setgrad_scaled(flat, grad_out, 1.0 / W)
+        self._clip_out(grad_out)
         return bits
 
 

@@ -521,3 +521,97 @@ def test_table_keeps_its_memory():
     other = [torch.full((1 << 20,), 9.0, device=DEV) for _ in range(4)]
     assert float(gcodec.grad_norm(g, INF)) == 2.0
     del other
+
+
+# ---------------------------------------------------------------------------
+# the reducers' options (one rank)
+# ---------------------------------------------------------------------------
+REDUCERS = [
+    ("QSGDMaxNormReducer", dict(quantization_level=4)),
+    ("QSGDMaxNormTwoScaleReducer", dict(lower_quantization_level=2, higher_quantization_level=4)),
+    ("QSGDMaxNormMultiScaleReducer", dict(quantization_levels=[2, 4, 6])),
+    ("GlobalRandKMaxNormReducer", dict(K=1000, quantization_level=4)),
+    ("GlobalRandKMaxNormTwoScaleReducer", dict(K=1000, lower_quantization_level=2, higher_quantization_level=4)),
+]
+STEP = [27, 64, 0, 1000, 3, 4099, 10, 70_001]
+
+
+def reducer(name, kw, **more):
+    return getattr(gcodec, name)(DEV, generator=gcodec.Generator(5, "philox"), **kw, **more)
+
+
+@pytest.mark.parametrize("name,kw", REDUCERS)
+def test_reducer_clips_what_it_writes(name, kw):
+    """max_grad_norm: the unclipped step's gradients, clipped; under the limit the same bits."""
+    ts = views(carve(STEP, [F32] * len(STEP), seed=121, scale=0.01))
+    plain, clipped, loose = ([torch.full_like(t, 9.0) for t in ts] for _ in range(3))
+    bits = reducer(name, kw).reduce(ts, plain)
+    r = reducer(name, kw, max_grad_norm=0.05)
+    assert r.grad_norm is None
+    assert r.reduce(ts, clipped) == bits
+    xs = f64(plain)
+    n = norm64(xs, 2)
+    assert n > 0.05
+    close_norm(r.grad_norm, n, roundings=5)
+    close_values(clipped, [x * coef64(n, 0.05) for x in xs], extra=8)
+    reducer(name, kw, max_grad_norm=2 * n).reduce(ts, loose)
+    for a, b in zip(plain, loose):
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+
+
+@pytest.mark.parametrize("name,kw", REDUCERS)
+def test_reducer_clips_what_it_sends(name, kw):
+    """local_max_norm: the bits of a step on gradients that clip_grads had clipped before."""
+    ts = views(carve(STEP, [F32] * len(STEP), seed=131, scale=0.01))
+    before = [torch.empty_like(t) for t in ts]
+    n = gcodec.clip_grads(ts, before, 0.05)
+    want, got = ([torch.full_like(t, 9.0) for t in ts] for _ in range(2))
+    bits = reducer(name, kw).reduce(before, want)
+    r = reducer(name, kw, local_max_norm=0.05)
+    assert r.reduce(ts, got) == bits and torch.equal(r.local_grad_norm, n)
+    for a, b in zip(want, got):
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+
+
+@pytest.mark.parametrize("name,kw", REDUCERS[:3])
+def test_reducer_on_bfloat16_gradients(name, kw):
+    """Both options take gradients of the smaller types (the codec itself is float32)."""
+    types = types_of("mixed", len(STEP))
+    ts, outs = views(carve(STEP, types, seed=141, scale=0.01)), views(carve(STEP, types, seed=142))
+    f = [t.float() for t in ts]
+    want = [torch.empty_like(t) for t in f]
+    reducer(name, kw, local_max_norm=0.5).reduce(f, want)
+    r = reducer(name, kw, local_max_norm=0.5, max_grad_norm=math.inf)
+    r.reduce(ts, outs)
+    close_norm(r.local_grad_norm, norm64(f64(ts), 2))
+    for a, b in zip(want, outs):
+        assert torch.equal(a.to(b.dtype), b)
+
+
+def test_reducer_step_captured_and_replayed():
+    """Local clipping, codec and clipped decode in one graph (Philox draws at a fixed offset)."""
+    ts, outs = views(carve(STEP, [F32] * len(STEP), seed=151, scale=0.01)), views(carve(STEP, [F32] * len(STEP), seed=152))
+    gi, go = gcodec.Grads(ts), gcodec.Grads(outs)
+    rng = gcodec.Generator(5, "philox").reserve(sum(STEP))
+
+    def step():
+        flat, peak, total = gcodec.flatten_clip(gi, 0.5)
+        words = codec.qsgd_encode(flat, peak, 8, rng)
+        return gcodec.qsgd_decode_clip(words, peak, 8, go, 0.3), total
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        n, total = step()
+    for _ in range(4):
+        with torch.no_grad():
+            for t in ts:
+                t.mul_(1.7)
+        g.replay()
+        torch.cuda.synchronize()
+        got, first = [o.clone() for o in outs], (float(n), float(total))
+        en, et = step()  # eager, on the same inputs
+        assert first == (float(en), float(et))
+        for a, b in zip(got, outs):
+            assert torch.equal(a, b)
