@@ -657,18 +657,19 @@ __device__ __forceinline__ uint64_t block_lanes(const LaneArg &a, float k, bool 
             q = quad_sum<P, true>(a, wd, i, full, a.L, mask, q);
             sum = lanes_join<P>(true, sum, (uint64_t)q);
         };
-        constexpr int U = 4;
-        for (; t + (U - 1) * stride < quads; t += U * stride) {
+        constexpr int U = 4;  // loads in flight, also for the last quads
+        for (; t < quads; t += U * stride) {
             uint4 wd[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                wd[u] = 4 * (t + u * stride) < a.cold ? ld_nt4u(words + t + u * stride) : words[t + u * stride];
+            for (int u = 0; u < U; ++u) {
+                const uint64_t j = min(t + u * stride, quads - 1);
+                wd[u] = 4 * j < a.cold ? ld_nt4u(words + j) : words[j];
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                add(wd[u], 4 * (t + u * stride));
+                if (t + u * stride < quads)
+                    add(wd[u], 4 * (t + u * stride));
         }
-        for (; t < quads; t += stride)
-            add(words[t], 4 * t);
     } else {
         Acc<P> real;
         for (; t < quads; t += stride) {
@@ -719,56 +720,117 @@ __device__ __forceinline__ void store_quad(uint64_t base, uint64_t start, uint64
             y[i + e - start] = Elem<T>::down(v[e]);
 }
 
-// Planes l0 .. l1 - 1 of tile t: of 256 kQuads consecutive words, a range of as
-// many flat elements each
+// A unit is planes l0 .. l1 - 1 of a tile of 256 kQuads consecutive words: of
+// each plane a range of as many flat elements.  Its words are loaded apart from
+// their use, ahead of what the block waits for.
 constexpr int kQuads = 2;
-__device__ __forceinline__ void decode_tile(const LaneArg &a, const GradRec *rd, uint32_t count, uint64_t t, uint32_t l0,
-                                            uint32_t l1, float k, float c)
-{
-    const uint32_t mask = a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u, lane = lane_id();
-    const uint64_t j0 = t * (256 * kQuads), j1 = min(j0 + 256 * kQuads, a.M);
+struct Unit {
+    uint64_t j0;
+    uint32_t l0, l1;
     uint4 wd[kQuads];
-#pragma unroll
-    for (int q = 0; q < kQuads; ++q) {
-        const uint64_t j = j0 + 256 * q + 4 * lane;  // M is a multiple of 4: a quad is in or out
-        wd[q] = j < j1 ? *reinterpret_cast<const uint4 *>(a.words + j) : make_uint4(0, 0, 0, 0);
-    }
-    for (uint32_t l = l0; l < l1; ++l) {
-        const uint64_t lo = (uint64_t)l * a.M + j0, hi = min((uint64_t)l * a.M + j1, a.n);
-        if (lo >= hi)
-            break;
-        grad_walk(rd, uni32(grad_find(rd, count, lo)), lo, hi, [&](uint32_t, uint32_t type, uint64_t base, uint64_t start, uint64_t pa, uint64_t pb) {
-#pragma unroll
-            for (int q = 0; q < kQuads; ++q) {
-                if (lo + 256 * q >= pb || lo + 256 * (q + 1) <= pa)
-                    continue;
-                const uint32_t we[4] = {wd[q].x, wd[q].y, wd[q].z, wd[q].w};
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int32_t Q = (int32_t)((we[e] >> (l * a.w)) & mask) - a.sub;
-                    const float d = k * (float)Q;
-                    v[e] = d * a.alpha * c;
-                }
-                const uint64_t i = lo + 256 * q + 4 * lane;
-                if (type == kTF32)
-                    store_quad<float>(base, start, pa, pb, i, v);
-                else if (type == kTBF16)
-                    store_quad<__bf16>(base, start, pa, pb, i, v);
-                else
-                    store_quad<_Float16>(base, start, pa, pb, i, v);
-            }
-        });
-    }
-}
+};
 
 __host__ __device__ __forceinline__ uint64_t decode_tiles(uint64_t M) { return (M + 256 * kQuads - 1) / (256 * kQuads); }
 
-// the planes of a tile in a.split shares
-__device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd, uint32_t count, uint64_t u, float k, float c)
+__device__ __forceinline__ Unit decode_load(const LaneArg &a, uint64_t u)
 {
-    const uint32_t per = (a.L + a.split - 1) / a.split, l0 = (uint32_t)(u % a.split) * per;
-    decode_tile(a, rd, count, u / a.split, l0, min(l0 + per, a.L), k, c);
+    Unit x;
+    const uint32_t per = (a.L + a.split - 1) / a.split;
+    x.j0 = u / a.split * (256 * kQuads);
+    x.l0 = (uint32_t)(u % a.split) * per;
+    x.l1 = min(x.l0 + per, a.L);
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        const uint64_t j = x.j0 + 256 * q + 4 * lane_id();  // M is a multiple of 4: a quad is in or out
+        x.wd[q] = j < a.M ? *reinterpret_cast<const uint4 *>(a.words + j) : make_uint4(0, 0, 0, 0);
+    }
+    return x;
+}
+
+struct DecodeArg {
+    float k, alpha, c;
+    int32_t sub;
+    uint32_t mask;
+};
+
+__device__ __forceinline__ void decode_quad(const DecodeArg &d, uint4 wd, uint32_t sh, float (&v)[4])
+{
+    const uint32_t we[4] = {wd.x, wd.y, wd.z, wd.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int32_t Q = (int32_t)((we[e] >> sh) & d.mask) - d.sub;
+        const float t = d.k * (float)Q;
+        v[e] = t * d.alpha * d.c;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void decode_whole(const DecodeArg &d, const Unit &x, uint32_t sh, Glob<T> y)
+{
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        float v[4];
+        decode_quad(d, x.wd[q], sh, v);
+        stv<T, 4>(y + (256 * q + 4 * lane_id()), v);
+    }
+}
+
+// Issue bound until the lookups were shared out: lane l finds plane l0 + l's
+// tensor (at most 32 planes), all at once, and a plane that lies whole in one
+// tensor is written without a test.
+__device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd, uint32_t count, const Unit &x, float k, float c)
+{
+    constexpr uint32_t kWords = 256 * kQuads;
+    const DecodeArg d{k, a.alpha, c, a.sub, a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u};
+    const uint32_t lane = lane_id();
+    if (x.l0 >= x.l1 || (uint64_t)x.l0 * a.M + x.j0 >= a.n)
+        return;
+    const uint64_t first = (uint64_t)min(x.l0 + lane, x.l1 - 1) * a.M + x.j0;
+    const uint32_t mine = x.l1 - x.l0 == 1 ? grad_find(rd, count, first)
+                          : first < a.n    ? grad_lane(rd, 0, count - 1, first)
+                                           : 0;
+    const uint64_t mpt = rd[mine].pt, mstart = rd[mine].start, mend = rd[mine + 1].start;
+    const uint32_t len = (uint32_t)min((uint64_t)kWords, a.M - x.j0);
+    for (uint32_t l = x.l0; l < x.l1; ++l) {
+        const uint64_t lo = (uint64_t)l * a.M + x.j0, hi = min(lo + len, a.n);
+        if (lo >= hi)
+            break;
+        const int at = (int)(l - x.l0);
+        auto of = [&](uint64_t v) {
+            return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), at) << 32 |
+                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, at);
+        };
+        const uint64_t pt = of(mpt), start = of(mstart), end = of(mend);
+        const uint32_t sh = l * a.w;
+        if (hi <= end && hi - lo == kWords) {
+            const uint64_t base = pt & 0x00ffffffffffffffull;
+            const uint32_t type = (uint32_t)(pt >> 56);
+            if (type == kTF32)
+                decode_whole<float>(d, x, sh, glob<float>(base, lo - start));
+            else if (type == kTBF16)
+                decode_whole<__bf16>(d, x, sh, glob<__bf16>(base, lo - start));
+            else
+                decode_whole<_Float16>(d, x, sh, glob<_Float16>(base, lo - start));
+            continue;
+        }
+        grad_walk(rd, (uint32_t)__builtin_amdgcn_readlane((int)mine, at), lo, hi,
+                  [&](uint32_t, uint32_t type, uint64_t base, uint64_t tstart, uint64_t pa, uint64_t pb) {
+#pragma unroll
+                      for (int q = 0; q < kQuads; ++q) {
+                          if (lo + 256 * q >= pb || lo + 256 * (q + 1) <= pa)
+                              continue;
+                          float v[4];
+                          decode_quad(d, x.wd[q], sh, v);
+                          const uint64_t i = lo + 256 * q + 4 * lane;
+                          if (type == kTF32)
+                              store_quad<float>(base, tstart, pa, pb, i, v);
+                          else if (type == kTBF16)
+                              store_quad<__bf16>(base, tstart, pa, pb, i, v);
+                          else
+                              store_quad<_Float16>(base, tstart, pa, pb, i, v);
+                      }
+                  });
+    }
 }
 
 template <int P, bool LDS>
@@ -776,12 +838,17 @@ __global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradAr
                                                                const uint64_t *__restrict__ part, uint32_t parts,
                                                                float *__restrict__ norm)
 {
-    const float k = *a.norm / a.s;
-    const bool exact = lanes_exact(a, k);
     __shared__ GradRec sd[LDS ? kLdsRecs + 1 : 1];
     __shared__ float sc;
     const GradRec *rd = LDS ? sd : dst.rec;
+    const uint64_t units = decode_tiles(a.M) * a.split, waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
+    uint64_t u = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id();
+    Unit x;
+    if (u < units)
+        x = decode_load(a, u);
+    const float k = *a.norm / a.s;
     if (wave_id() == 0) {
+        const bool exact = lanes_exact(a, k);
         uint64_t sum = 0;  // the bits of 0.0 as well
         for (uint32_t i = lane_id(); i < parts; i += 64)
             sum = lanes_join<P>(exact, sum, part[i]);
@@ -796,9 +863,12 @@ __global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradAr
         stage_table(dst, sd);
     __syncthreads();
     const float c = sc;
-    const uint64_t units = decode_tiles(a.M) * a.split, waves = (uint64_t)gridDim.x * (kScaleThreads / 64);
-    for (uint64_t u = (uint64_t)blockIdx.x * (kScaleThreads / 64) + wave_id(); u < units; u += waves)
-        decode_unit(a, rd, dst.count, u, k, c);
+    while (u < units) {
+        decode_unit(a, rd, dst.count, x, k, c);
+        u += waves;
+        if (u < units)
+            x = decode_load(a, u);
+    }
 }
 
 // both passes in one block
@@ -820,7 +890,7 @@ __global__ __launch_bounds__(kNormThreads) void k_decode_clip_one(LaneArg a, Gra
     }
     __syncthreads();
     for (uint64_t u = wave_id(), units = decode_tiles(a.M) * a.split; u < units; u += kNormThreads / 64)
-        decode_unit(a, sd, dst.count, u, k, sc);
+        decode_unit(a, sd, dst.count, decode_load(a, u), k, sc);
 }
 
 // ---------------------------------------------------------------------------
