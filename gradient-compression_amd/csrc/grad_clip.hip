@@ -19,9 +19,12 @@
 // and one fused multiply-add for each element are about a seventh of the
 // vector unit's time at the rate that the memory delivers float32.
 //
-// All of it is bound by HBM: norm reads the gradients once; clip reads them
-// twice and writes them once, the second read walking backwards so that what
-// the first read last is still in the 256 MB of cache in front of the memory.
+// All of it is bound by HBM.  The norm reads the gradients once, clipping reads
+// them twice and writes them once; of a list beyond the 256 MB of cache in front
+// of the memory, the first read passes all but the end by the cache, and the
+// second finds that end there.  Short lists are bound by the two launches and
+// the chain partials -> c -> first load inside the second: 8.3 us for 10,000 to
+// a million elements, whatever their number.
 #include "gc_device.h"
 #include "gc_host.h"
 #include "grads.h"
@@ -33,18 +36,42 @@
 
 namespace gc {
 
-constexpr uint32_t kTile = 2048;       // flat elements a wave takes at a time, at most
+// Flat elements a wave takes at a time, at most: 8 KB of float32 (eight vectors
+// a lane).  16-bit lists take twice as many in the norm: 426M bfloat16 139 us
+// against 149 at 2048; float32 loses by it (1e9: 588 against 579).
+constexpr uint32_t kTile = 2048;
+constexpr uint32_t kLeastTile = 256;  // a vector of float32 a lane
+
+// Two blocks a CU, 32 waves of 4 KB in flight each.  256 / 512 / 1024 blocks:
+// 18.7 / 17.4 / 18.6 us on 94 MB of float32.
 constexpr unsigned kNormThreads = 1024;
-constexpr unsigned kNormGrid = 512;    // two blocks a CU: 32 waves, each with 4 KB in flight
+constexpr unsigned kNormGrid = 512;
+
+// The pass that writes runs best with about a tile a wave, in small blocks that
+// come and go (2048 / 16384 blocks: 474 / 437 us on 426M bfloat16), but where
+// all tiles are under way at once, fewer and larger blocks form c fewer times
+// (14.7M float32: 38.0 us in blocks of 256, 34.7 in blocks of 1024; at 426M
+// elements 387 and 416).
 constexpr unsigned kScaleThreads = 256;
 constexpr unsigned kScaleGrid = 16384;
+constexpr uint64_t kWaves = 8192;  // resident at once: 256 CUs of 32
+
+// Words: one block a CU adds them (128 / 256 / 512 blocks: 33.3 / 30.9 / 32.5 us
+// with the decode, whose every block reads the partials), 4096 decode them
+// (2048 / 4096 / 8192: 285 / 258 / 260 us for 246M elements).
 constexpr unsigned kLaneGrid = 256;
 constexpr unsigned kDecodeGrid = 4096;
-constexpr uint64_t kWaves = 8192;      // resident at once: 256 CUs of 32
-constexpr uint64_t kOneElems = 8192;   // what one block does alone
-constexpr uint32_t kLeastTile = 256;   // a vector a lane
-constexpr uint64_t kFewElems = 1024;   // tensors of fewer elements are small
-constexpr uint64_t kFewEach = 64;      // for each tensor's own norm
+
+// What one block does alone (one_block) and the average sizes below which
+// tensors count as small: for the sums and the scaling of a list, and for
+// each tensor's own norm.
+constexpr uint64_t kOneElems = 8192;
+constexpr uint64_t kFewElems = 1024;
+constexpr uint64_t kFewEach = 64;
+
+// The cache in front of HBM.  Clipping 426M bfloat16 takes 374 us with the last
+// 256 MB read through it, 377 with 192, 394 with 320, 404 with none, and 437
+// with everything.
 constexpr uint64_t kCacheBytes = 256ull << 20;
 constexpr double kEps = 1e-6;
 
@@ -102,7 +129,8 @@ __device__ __forceinline__ void wave_join(A &a)
         a.join(a.shuffled(m));
 }
 
-// the wave's elements x[0 .. cnt), x and cnt the same for all lanes
+// the wave's elements x[0 .. cnt), x and cnt the same for all lanes; NT: past
+// the cache (1e9 float32 in 577 us, 6.9 TB/s, against 645 through it)
 template <class T, bool NT, class F>
 __device__ __forceinline__ void wave_read(Glob<const T> x, uint32_t cnt, F f)
 {
@@ -146,7 +174,9 @@ __device__ __forceinline__ void wave_read_any(uint32_t type, uint64_t base, uint
 }
 
 // f(i, x) for element lo + i of a tile of kLeastTile or fewer elements of
-// tensors s0 .. s1, the lane's own: four lookups, then four loads in flight
+// tensors s0 .. s1, the lane's own: four lookups, then four loads in flight.
+// Clipping 5000 elements of 500 tensors takes 14.3 us so, 83.8 when each tensor
+// is waited for.
 template <class F>
 __device__ __forceinline__ void lane_read(const GradRec *rec, uint32_t s0, uint32_t s1, uint64_t lo, uint64_t hi, F f)
 {
@@ -329,7 +359,12 @@ __device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, uint
         each[s] = (float)root_of(P, t);
 }
 
-// One partial a block; a grid of one block finishes the call itself
+// The norm's first pass: one partial a block; a grid of one block finishes the
+// call itself.  A block's tiles are 16 consecutive ones of every gridDim.x * 16,
+// so the chip reads a few MB of consecutive addresses at any time.  Bound by
+// HBM: 4 GB of float32 in 579 us (6.9 TB/s), 853 MB of bfloat16 in 125 us
+// (6.8 TB/s; 132 us with each tensor's norm); 94 MB of float32 in 17 us, of which
+// 4 us are the launch and the first loads.
 template <int P, bool EACH, bool PEAK, bool LDS>
 __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, uint32_t tile, uint64_t cold,
                                                                double *__restrict__ part,
@@ -358,7 +393,9 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
             tensor_norm<P, 1>(rec, s, tile, slots, each);
 }
 
-// block 0: the total and N; block 1 + s: the norm of tensor s
+// The norm's second pass, over the partials.  Block 0: the total and N; block
+// 1 + s: the norm of tensor s.  Latency: 2 us queued behind the first pass; 6 us
+// with each norm, where the largest tensor has 16,000 slots.
 template <int P>
 __global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, uint32_t tile, const double *__restrict__ part, uint32_t parts,
                                                               const double *__restrict__ slots,
@@ -460,8 +497,13 @@ __device__ __forceinline__ void scale_tile(const GradRec *rs, const GradRec *rd,
     });
 }
 
-// The partials' pass has c = 1 in most steps of a training run; in place
-// nothing is left to do then.
+// Clipping's second pass.  In place with c = 1, as in most steps of a training
+// run, nothing is left to do.  Tiles in the order of the norm: backwards, to
+// meet the cache's content first, is no faster (426M bfloat16 380 us against 370,
+// 23.5M float32 into a bucket 49.8 against 48.5).  Stores pass the cache: through
+// it, what the first pass left there is lost (351 -> 382 us, 246M bfloat16 into a
+// bucket).  Bound by HBM: 1.7 GB in 248 us (6.9 TB/s, a part from the cache);
+// 118 MB of 14.7M float32 in 22 us, 188 MB of 23.5M into a bucket in 31 us.
 template <bool FLAT, bool LDS>
 __global__ __launch_bounds__(kNormThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n, uint32_t tile,
                                                               uint64_t cold, int p,
@@ -514,7 +556,8 @@ __global__ __launch_bounds__(kNormThreads) void k_grad_scale(GradArg src, GradAr
     }
 }
 
-// both passes in one block
+// Both passes in one block, without a second launch: 5.6 us for 1000 elements
+// of 3 tensors.  Latency of two rounds of loads.
 template <int P, bool FLAT>
 __global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, GradArg dst, float *flat, uint64_t n,
                                                                 uint32_t tile, double max_norm, bool in_place,
@@ -695,6 +738,10 @@ __device__ __forceinline__ uint64_t block_lanes(const LaneArg &a, float k, bool 
     return sum;
 }
 
+// The words' first pass: 1/6 (4 bit, one rank) to 1/2 (8 bit, eight ranks) of what
+// reading the decoded float32 gradients would take.  Bound by HBM where there are many
+// (491 MB in 75 us, 6.5 TB/s); 15.7 MB take 8 us, half of it the launch and the
+// first loads.
 template <int P>
 __global__ __launch_bounds__(kNormThreads) void k_lane_norm(LaneArg a, uint64_t *__restrict__ part)
 {
@@ -833,6 +880,11 @@ __device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd,
     }
 }
 
+// The words' second pass: the gradients are written once, clipped.  A thread
+// holds two quads of words and writes them plane by plane, so every access of a
+// wave is 1 KB (float32) or 512 bytes of consecutive addresses.  Bound by HBM
+// for many (491 MB in and 491 MB out in 175 us, 5.6 TB/s); 23.5M float32 at
+// 4 bits, 110 MB, take 20 us, of which 5 are the launch and the chain to c.
 template <int P, bool LDS>
 __global__ __launch_bounds__(kScaleThreads) void k_decode_clip(LaneArg a, GradArg dst, double max_norm,
                                                                const uint64_t *__restrict__ part, uint32_t parts,
@@ -1043,7 +1095,7 @@ static uint32_t norm_tile(const gc_grads *g, bool each = false)
 static unsigned norm_grid(uint64_t n, uint64_t count, uint32_t tile)
 {
     const uint64_t tiles = (n + tile - 1) / tile, per = kNormThreads / 64;
-    return one_block(n, count) ? 1u : (unsigned)std::min<uint64_t>((tiles + per - 1) / per, kNormGrid);
+    return one_block(n, count) ? 1u : (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
 }
 
 // of `of` elements or words that take `bytes`, those ahead of the last kCacheBytes

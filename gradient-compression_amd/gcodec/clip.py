@@ -89,7 +89,8 @@ class Grads:
 
     It keeps the tensors' memory alive, not their shapes or later replacements:
     a gradient that is replaced by another tensor needs another table, and a
-    storage that is resized under a table must not be used through it."""
+    storage that is resized under a table must not be used through it.  A
+    captured call needs its table for as long as the graph is replayed."""
 
     def __init__(self, tensors):
         tensors = list(tensors)
@@ -155,14 +156,19 @@ class Grads:
         return torch.empty((), dtype=dtype, device=self.device)
 
 
-def _table(grads, ordered=True) -> Grads:
+def _table(grads, ordered=True, written=False) -> Grads:
+    """The table of a list (written: whose tensors this call writes; autograd is told)."""
     if isinstance(grads, Grads):
         return grads
     if isinstance(grads, torch.Tensor):
         grads = [grads]
-    g = Grads._of_call(grads if isinstance(grads, (list, tuple)) else list(grads), False, ordered)
+    elif not isinstance(grads, (list, tuple)):
+        grads = list(grads)
+    g = Grads._of_call(grads, False, ordered)
     if g is None:
         _refuse("Grads: empty tensor list")
+    if written:
+        _lib.tensor_list().written(grads, False)
     return g
 
 
@@ -235,8 +241,8 @@ def clip_grads(grads, out, max_norm: float, norm_type: float = 2.0, error_if_non
     tensor may be clipped onto itself; apart from that the tensors of `out`
     share no memory with each other or with `grads`."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
-    src = _table(grads)
-    dst = src if out is grads else _table(out)
+    src = _table(grads, written=out is grads)
+    dst = src if out is grads else _table(out, written=True)
     return _clip(src, dst, max_norm, code, error_if_nonfinite, group, "clip_grads")
 
 
@@ -288,7 +294,7 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     before clipping.  The unclipped gradients are never stored."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     dev = _on_gpu(words)
-    g = _table(grads)
+    g = _table(grads, written=True)
     if dev != g.device:
         _refuse(f"qsgd_decode_clip: words on {dev}, gradients on {g.device}")
     if words.dtype != torch.int32 or not words.is_contiguous():

@@ -41,6 +41,10 @@ LISTS = {
     "ragged": RAGGED,
     "one block's": [32_767, 2],
     "tiny, past the LDS table": [i % 8 for i in range(1500)],
+    "only empty, past the LDS table": [0] * 1100,
+    "many, past the LDS table": [1500 + i % 9 for i in range(1100)],
+    "small": [83 + 7 * (i % 5) for i in range(120)],
+    "small among large": [300_000] + [40] * 300 + [70_001, 0, 5],
     "several blocks": [1_000_003, 12, 2_000_001],
 }
 UNIT = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
@@ -197,10 +201,12 @@ def test_clip_list_to_list(name, kind, p, factor):
     xs = f64(views(src))
     n = norm64(xs, p)
     m = factor * n if n else 1.0
+    version = views(dst)[0]._version
     total = gcodec.clip_grads(views(src), views(dst), m, p)
     close_norm(total, n)
     close_values(views(dst), [x * coef64(n, m) for x in xs])
     guards_hold(dst)
+    assert views(dst)[0]._version > version  # autograd sees the write
     for x, t in zip(xs, views(src)):
         assert np.array_equal(x, t.cpu().double().numpy())  # read only
 
@@ -383,7 +389,8 @@ def packed(n, bits, world, seed, norm=0.02):
 @pytest.mark.parametrize("bits,world,p", [(1, 1, 2), (2, 1, 1), (4, 1, 2), (4, 1, INF), (4, 3, 2), (8, 8, 2), (8, 1, 1),
                                           (12, 2, 2), (16, 8, 2), (20, 1, 1), (24, 1, INF)])
 @pytest.mark.parametrize("name,kind", [("one", "fp32"), ("empty ends", "bf16"), ("ragged", "mixed"), ("ragged", "fp32"),
-                                       ("tiny, past the LDS table", "fp16"), ("several blocks", "bf16")])
+                                       ("tiny, past the LDS table", "fp16"), ("several blocks", "bf16"),
+                                       ("many, past the LDS table", "mixed"), ("small among large", "mixed")])
 def test_decode(name, kind, bits, world, p, factor):
     sizes = LISTS[name]
     n = sum(sizes)
