@@ -382,7 +382,8 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
     Acc<kPInf> top;
     block_norm<P, EACH, PEAK>(rec, g.count, n, tile, cold, slots, all, top);
     if (threadIdx.x == 0) {
-        part[blockIdx.x] = all.value();
+        if (part)
+            part[blockIdx.x] = all.value();
         if (PEAK)
             peak[blockIdx.x] = top.m;
         if (gridDim.x == 1)
@@ -1084,6 +1085,7 @@ static uint32_t tile_of(uint64_t n, uint64_t count, uint32_t most, uint64_t few 
 // takes 6.3 / 11.6 / 18.3 us in one block and 8.3 / 11.1 / 13.4 us in two
 // launches, 20000 of 3 / 60 tensors 8.8 / 19.2 and 9.5 / 11.1 us.
 static bool one_block(uint64_t n, uint64_t count) { return n + 8 * count <= kOneElems; }
+static_assert(kOneElems / 8 <= kLdsRecs, "one block's table is in LDS");
 
 // The norm's tile: up to 8 KB of gradients.  Each tensor's own norm takes a
 // lane a tensor there, one element after the other, so only the smallest.
@@ -1112,6 +1114,13 @@ static uint32_t split_of(uint64_t tiles, uint32_t L)
     return tiles >= want ? 1u : (uint32_t)std::min<uint64_t>(L, (want + tiles - 1) / std::max<uint64_t>(tiles, 1));
 }
 
+static int check_workspace(const gc_grads *g, bool each, const void *workspace, const char *what)
+{
+    GC_REQUIRE(workspace || gc_grad_workspace_size(g->n, g->count, each) == 0, "%s: null workspace", what);
+    GC_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: misaligned workspace", what);
+    return GC_OK;
+}
+
 // f(p as a constant)
 template <class F>
 static void with_p(uint32_t p, F f)
@@ -1131,10 +1140,10 @@ static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, 
     const GradArg a = arg_of(g);
     const uint32_t tile = norm_tile(g, EACH);
     const dim3 grid(norm_grid(g->n, g->count, tile)), block(kNormThreads);
-    char *w = static_cast<char *>(ws);
+    char *w = static_cast<char *>(ws);  // null: one block, which leaves nothing there
     double *part = reinterpret_cast<double *>(w);
-    uint32_t *peak = reinterpret_cast<uint32_t *>(w + kWsPeak);
-    double *slots = reinterpret_cast<double *>(w + kWsSlots);
+    uint32_t *peak = w ? reinterpret_cast<uint32_t *>(w + kWsPeak) : nullptr;
+    double *slots = w ? reinterpret_cast<double *>(w + kWsSlots) : nullptr;
     with_p(p, [&](auto P) {
         if (g->count <= kLdsRecs)
             hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, tile, cold, part, peak, slots,
@@ -1232,6 +1241,8 @@ int gc_grads_fill(const gc_grads *grads, uint64_t *rec, gc_stream_t stream)
 
 size_t gc_grad_workspace_size(uint64_t n, uint64_t count, int each)
 {
+    if (!each && one_block(n, count))
+        return 0;
     return kWsSlots + (each ? (n / tile_of(n, count, kTile, kFewEach) + 1 + count) * sizeof(double) : 0);
 }
 
@@ -1242,7 +1253,8 @@ int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, 
     int rc;
     if ((rc = check_grads(grads, what)) || (rc = check_p(p, what)))
         return rc;
-    GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
+    if ((rc = check_workspace(grads, each != nullptr, workspace, what)))
+        return rc;
     hipStream_t st = as_stream(stream);
     if (each)
         launch_norm<true, false>(grads, p, ~0ull, workspace, total, norm, each, st);
@@ -1293,10 +1305,10 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
     }
     if (!same && (rc = check_apart(src, dst, what)))
         return rc;
-    GC_REQUIRE(total || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0),
-               "%s: null or misaligned workspace", what);
+    if (!total && (rc = check_workspace(src, false, workspace, what)))
+        return rc;
     hipStream_t st = as_stream(stream);
-    if (!total && src->count <= kLdsRecs && one_block(src->n, src->count)) {
+    if (!total && one_block(src->n, src->count)) {
         with_p(p, [&](auto P) {
             hipLaunchKernelGGL((k_grad_clip_one<P(), false>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), arg_of(dst),
                                nullptr, src->n, tile_of(src->n, src->count, kTile), max_norm, same, norm, nullptr);
@@ -1329,7 +1341,8 @@ int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double ma
         return rc;
     GC_REQUIRE(peak && (src->n == 0 || flat) && (reinterpret_cast<uintptr_t>(flat) & 3u) == 0,
                "%s: null or misaligned output", what);
-    GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
+    if ((rc = check_workspace(src, false, workspace, what)))
+        return rc;
     const uint64_t lo = reinterpret_cast<uint64_t>(flat), hi = lo + 4 * src->n;
     for (uint64_t s = 0; s < src->count; ++s) {
         const Span x = span_of(src, s);
@@ -1337,7 +1350,7 @@ int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double ma
                    (unsigned long long)s);
     }
     hipStream_t st = as_stream(stream);
-    if (src->count <= kLdsRecs && one_block(src->n, src->count)) {
+    if (one_block(src->n, src->count)) {
         with_p(p, [&](auto P) {
             hipLaunchKernelGGL((k_grad_clip_one<P(), true>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), GradArg{}, flat,
                                src->n, tile_of(src->n, src->count, kTile), max_norm, false, norm, peak);
@@ -1376,7 +1389,8 @@ int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, ui
                (unsigned long long)n);
     GC_REQUIRE(norm && total_norm && (n == 0 || words), "%s: null pointer", what);
     GC_REQUIRE(aligned16(words), "%s: words must be 16-byte aligned", what);
-    GC_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: null or misaligned workspace", what);
+    if ((rc = check_workspace(dst, false, workspace, what)))
+        return rc;
     uint64_t at = 0;
     const uint64_t w0 = reinterpret_cast<uint64_t>(words), m0 = reinterpret_cast<uint64_t>(norm);
     GC_REQUIRE(!meets(dst, {w0, w0 + 4 * lanes->plane_words}, &at) && !meets(dst, {m0, m0 + 4}, &at),
@@ -1391,7 +1405,7 @@ int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, ui
     const GradArg d = arg_of(dst);
     const dim3 grid(grid_of(decode_tiles(lanes->plane_words) * a.split, kScaleThreads, kDecodeGrid));
     with_p(p, [&](auto P) {
-        if (dst->count <= kLdsRecs && n <= kOneElems) {
+        if (one_block(n, dst->count)) {
             hipLaunchKernelGGL(k_decode_clip_one<P()>, dim3(1), dim3(kNormThreads), 0, st, a, d, max_norm, total_norm);
             return;
         }

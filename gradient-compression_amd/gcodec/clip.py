@@ -73,6 +73,10 @@ def _call(name: str, device, *args):
         raise _lib.GCodecError(rc, f"{name}: {_lib.last_error()}")
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def _on_gpu(t: torch.Tensor) -> torch.device:
     """t's device, always with its index."""
     dev = _dev(t)
@@ -139,6 +143,7 @@ class Grads:
         if self.device is None:
             self.device = _DEVICES[index] = torch.device("cuda", index)
         self.count, self.n = self.struct.count, self.struct.n
+        self._ws = lib.gc_grad_workspace_size(self.n, self.count, 0)
         return True
 
     def _use(self):
@@ -148,9 +153,10 @@ class Grads:
                 self._rec.record_stream(torch.cuda.current_stream(self.device))
         return self._ref
 
-    def _workspace(self, each: bool = False) -> torch.Tensor:
-        size = _lib.load().gc_grad_workspace_size(self.n, self.count, each)
-        return torch.empty(size, dtype=torch.uint8, device=self.device)
+    def _workspace(self, each: bool = False):
+        """A call's workspace, or None where it needs none."""
+        size = _lib.load().gc_grad_workspace_size(self.n, self.count, 1) if each else self._ws
+        return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
 
     def _scalar(self, dtype=torch.float32) -> torch.Tensor:
         return torch.empty((), dtype=dtype, device=self.device)
@@ -194,8 +200,7 @@ def _finite(norm: torch.Tensor, what: str):
 
 def _norm_into(g: Grads, code: int, norm, each=None, total=None):
     ws = g._workspace(each is not None)
-    _call("gc_grad_norm", g.device, g._use(), code, total.data_ptr() if total is not None else None,
-          norm.data_ptr() if norm is not None else None, each.data_ptr() if each is not None else None, ws.data_ptr())
+    _call("gc_grad_norm", g.device, g._use(), code, _at(total), _at(norm), _at(each), _at(ws))
 
 
 def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False, error_if_nonfinite: bool = False, group=None):
@@ -231,7 +236,7 @@ def _clip(src: Grads, dst: Grads, max_norm: float, code: int, error_if_nonfinite
             _finite(norm, what)
     ws = src._workspace()
     _call("gc_grad_clip", src.device, src._use(), dst._use(), code, max_norm,
-          total.data_ptr() if total is not None else None, norm.data_ptr(), ws.data_ptr())
+          _at(total), norm.data_ptr(), _at(ws))
     return norm
 
 
@@ -283,7 +288,7 @@ def flatten_clip(grads, max_norm: float, norm_type: float = 2.0, flat=None):
     norm = g._scalar()
     ws = g._workspace()
     _call("gc_grad_flatten_clip", g.device, g._use(), flat.data_ptr(), code, max_norm, peak.data_ptr(), norm.data_ptr(),
-          ws.data_ptr())
+          _at(ws))
     return flat, peak, norm
 
 
@@ -308,5 +313,5 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     out = g._scalar()
     ws = g._workspace()
     _call("gc_qsgd_decode_clip", dev, words.data_ptr(), g.n, nt.data_ptr(), int(bits), C.byref(lanes), float(alpha),
-          g._use(), code, max_norm, out.data_ptr(), ws.data_ptr())
+          g._use(), code, max_norm, out.data_ptr(), _at(ws))
     return out

@@ -83,6 +83,7 @@ def clip_call(src, dst, p=2, max_norm=1.0, total=None, norm=NORM, ws=WS):
 
 def test_clip_refuses_what_would_race_or_misread():
     a = Table([4, 8], [0x1000, 0x2000], [F32, F16])
+    big = Table([9000], [0x80000], [F32])
     for bad, msg in [
         (Table([4], [0x3000], [F32]), "tensors into"),
         (Table([4, 9], [0x3000, 0x4000], [F32, F16]), "sizes"),
@@ -94,7 +95,7 @@ def test_clip_refuses_what_would_race_or_misread():
         assert clip_call(a, bad) == _lib.GC_EINVAL and msg in err(), err()
     twice = Table([4, 4], [0x1000, 0x1000], [F32, F32])
     assert clip_call(twice, twice) == _lib.GC_EINVAL and "share memory" in err()
-    assert clip_call(a, a, ws=None) == _lib.GC_EINVAL and "workspace" in err()
+    assert clip_call(big, big, ws=None) == _lib.GC_EINVAL and "workspace" in err()
     assert clip_call(a, a, ws=WS + 4) == _lib.GC_EINVAL and "workspace" in err()
     assert clip_call(a, a, p=3) == _lib.GC_EINVAL and "GC_NORM_INF" in err()
     for m in (-1.0, math.nan, -math.inf):
@@ -107,7 +108,10 @@ def test_norm_and_flatten_refuse():
     lib = _lib.load()
     a = Table([4, 8], [0x1000, 0x2000], [F32, F16])
     assert lib.gc_grad_norm(a.ref, 7, None, NORM, None, WS, None) == _lib.GC_EINVAL
-    assert lib.gc_grad_norm(a.ref, 2, None, NORM, None, None, None) == _lib.GC_EINVAL
+    assert lib.gc_grad_norm(a.ref, 2, None, NORM, NORM, None, None) == _lib.GC_EINVAL and "workspace" in err()
+    assert lib.gc_grad_norm(a.ref, 2, None, NORM, None, WS + 4, None) == _lib.GC_EINVAL and "workspace" in err()
+    assert lib.gc_grad_workspace_size(12, 2, 0) == 0 < lib.gc_grad_workspace_size(12, 2, 1)
+    assert lib.gc_grad_workspace_size(12, 1100, 0) > 0 and lib.gc_grad_workspace_size(9000, 1, 0) > 0
     assert lib.gc_grad_norm(None, 2, None, NORM, None, WS, None) == _lib.GC_EINVAL
     assert lib.gc_grad_norm_root(None, 2, NORM, None) == _lib.GC_EINVAL
     flat = lib.gc_grad_flatten_clip
@@ -128,7 +132,7 @@ def test_decode_refuses():
             assert lib.gc_qsgd_layout(n, bits, 1, C.byref(ln)) == 0
         return lib.gc_qsgd_decode_clip(words, n, norm, bits, C.byref(ln), 1.0, g.ref, p, m, out, ws, None)
 
-    for kw in (dict(n=13), dict(words=None), dict(words=0x8004), dict(norm=None), dict(out=None), dict(ws=None),
+    for kw in (dict(n=13), dict(words=None), dict(words=0x8004), dict(norm=None), dict(out=None), dict(ws=WS + 4),
                dict(p=5), dict(m=math.nan), dict(words=0x2000), dict(norm=0x1004)):
         assert call(a, **kw) == _lib.GC_EINVAL, kw
     other = _lib.gc_lanes()

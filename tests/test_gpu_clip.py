@@ -622,3 +622,49 @@ def test_reducer_step_captured_and_replayed():
         assert first == (float(en), float(et))
         for a, b in zip(got, outs):
             assert torch.equal(a, b)
+
+
+def test_ranks_clip_their_shards_by_the_whole():
+    import os
+    import tempfile
+
+    import torch.multiprocessing as mp
+
+    import _clip_workers as W
+
+    with tempfile.TemporaryDirectory() as td:
+        mp.spawn(W.clip_shards, args=(2, os.path.join(td, "init"), td), nprocs=2, join=True)
+        r = [dict(np.load(os.path.join(td, f"r{k}.npz"), allow_pickle=False)) for k in range(2)]
+    parts = [[s.double().numpy() for s in W.shards(k, 2)] for k in range(2)]
+    for p in (1.0, 2.0, INF):
+        n = norm64(parts[0] + parts[1], p)
+        for k in range(2):
+            close_norm(r[k][f"norm/{p}"], n)
+            close_norm(r[k][f"clip/{p}"], n)
+            close_values([torch.from_numpy(r[k][f"grads/{p}"])], [np.concatenate(parts[k]) * coef64(n, 0.75)])
+    for k in range(2):
+        assert float(r[k]["alone"]) == 6.0 and np.isnan(r[k]["nan"]).all()
+
+
+def test_checked_calls_clip_alike():
+    """error_if_nonfinite takes the norm in a call of its own: the same bits follow."""
+    ts = views(carve(RAGGED, types_of("mixed", len(RAGGED)), seed=161))
+    a, b = ([torch.zeros_like(t) for t in ts] for _ in range(2))
+    na = gcodec.clip_grads(ts, a, 1.0)
+    nb = gcodec.clip_grads(ts, b, 1.0, error_if_nonfinite=True)
+    assert torch.equal(na, nb) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_lists_on_another_stream():
+    """Lists made, used and dropped on a stream of their own, over and over."""
+    s = torch.cuda.Stream()
+    want = None
+    with torch.cuda.stream(s):
+        for _ in range(30):
+            ts = [torch.full((5000 + i,), 0.5, device=DEV, dtype=(F32, BF16)[i % 2]) for i in range(40)]
+            got = gcodec.clip_grads(ts, ts, 1.0)
+            flat, peak, after = gcodec.flatten_clip(ts, 10.0)
+            res = torch.stack([got, after, peak[0]])
+            want = res if want is None else want
+            del ts, flat
+            assert torch.equal(res, want)
