@@ -49,12 +49,14 @@ constexpr unsigned kNormGrid = 512;
 
 // The pass that writes runs best with about a tile a wave, in small blocks that
 // come and go (2048 / 16384 blocks: 474 / 437 us on 426M bfloat16), but where
-// all tiles are under way at once, fewer and larger blocks form c fewer times
-// (14.7M float32: 38.0 us in blocks of 256, 34.7 in blocks of 1024; at 426M
-// elements 387 and 416).
+// most tiles are under way at once, fewer and larger blocks form c fewer times
+// (14.7M float32: 33.7 us in blocks of 256, 32.4 in blocks of 1024; at 426M
+// elements 387 and 416).  Both passes of a list of up to kSpread tiles go in
+// small blocks again, over more CUs (60,000 elements of 3 tensors 8.8 -> 7.9 us).
 constexpr unsigned kScaleThreads = 256;
 constexpr unsigned kScaleGrid = 16384;
 constexpr uint64_t kWaves = 8192;  // resident at once: 256 CUs of 32
+constexpr uint64_t kSpread = 1024;
 
 // Words: one block a CU adds them (128 / 256 / 512 blocks: 33.3 / 30.9 / 32.5 us
 // with the decode, whose every block reads the partials), 4096 decode them
@@ -68,6 +70,12 @@ constexpr unsigned kDecodeGrid = 4096;
 constexpr uint64_t kOneElems = 8192;
 constexpr uint64_t kFewElems = 1024;
 constexpr uint64_t kFewEach = 64;
+
+// The tensors of a tile beyond which lanes take their own: 3 / 5 for clipping
+// 120,000 elements of 500 tensors 12.2 / 13.0 us, for each norm of a million of 300
+// 15.5 / 12.0.
+constexpr uint32_t kMany = 3;
+constexpr uint32_t kManyEach = 5;
 
 // The cache in front of HBM.  Clipping 426M bfloat16 takes 374 us with the last
 // 256 MB read through it, 377 with 192, 394 with 320, 404 with none, and 437
@@ -196,23 +204,24 @@ __device__ __forceinline__ void lane_read(const GradRec *rec, uint32_t s0, uint3
             f(u * 64 + lane_id(), x[u]);
 }
 
-// The block's share of the sum of |x|^p and (PEAK) of max |x|, valid in thread 0.
+// The share of a block of `per` waves of the sum of |x|^p and (PEAK) of max |x|, valid in thread 0.
 // EACH: also the sum of every piece, at slot (tile + tensor): along the flat
 // sequence each next piece has the next tile or the next tensor, so a tensor's
 // pieces have consecutive slots of their own.
 template <int P, bool EACH, bool PEAK>
-__device__ __forceinline__ void block_norm(const GradRec *rec, uint32_t count, uint64_t n, uint32_t tile, uint64_t cold,
+__device__ __forceinline__ void block_norm(uint32_t per, const GradRec *rec, uint32_t count, uint64_t n, uint32_t tile,
+                                           uint64_t cold,
                                            double *__restrict__ slots,
                                            Acc<P> &all, Acc<kPInf> &top)
 {
     __shared__ double sacc[kNormThreads / 64];
     __shared__ uint32_t smax[kNormThreads / 64];
     __shared__ double svals[EACH ? kNormThreads / 64 : 1][EACH ? kLeastTile : 1];
-    const uint64_t waves = (uint64_t)gridDim.x * (kNormThreads / 64);
-    for (uint64_t t = (uint64_t)blockIdx.x * (kNormThreads / 64) + wave_id(); t * tile < n; t += waves) {
+    const uint64_t waves = (uint64_t)gridDim.x * per;
+    for (uint64_t t = (uint64_t)blockIdx.x * per + wave_id(); t * tile < n; t += waves) {
         const uint64_t lo = t * tile, hi = min(lo + tile, n);
         const uint32_t s0 = uni32(grad_find(rec, count, lo));
-        if (tile == kLeastTile && grad_many(rec, count, s0, hi)) {
+        if (tile == kLeastTile && grad_many(rec, count, s0, hi, EACH ? kManyEach : kMany)) {
             const uint32_t s1 = uni32(grad_find(rec, count, hi - 1));
             double *v = EACH ? svals[wave_id()] : nullptr;
             lane_read(rec, s0, s1, lo, hi, [&](uint32_t i, float x) {
@@ -229,10 +238,17 @@ __device__ __forceinline__ void block_norm(const GradRec *rec, uint32_t count, u
                 for (uint32_t s = s0 + lane_id(); s <= s1; s += 64) {
                     const uint64_t a = max(rec[s].start, lo), b = min(rec[s + 1].start, hi);
                     Acc<P> one;
-                    for (uint64_t e = a; e < b; ++e) {
-                        Acc<P> o;
-                        o.set(v[e - lo]);
-                        one.join(o);
+                    for (uint64_t e = a; e < b; e += 8) {  // eight reads in flight; 0 joins without effect
+                        double x[8];
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k)
+                            x[k] = e + k < b ? v[e + k - lo] : 0.0;
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) {
+                            Acc<P> o;
+                            o.set(x[k]);
+                            one.join(o);
+                        }
                     }
                     if (a < b)
                         slots[t + s] = one.value();
@@ -272,7 +288,7 @@ __device__ __forceinline__ void block_norm(const GradRec *rec, uint32_t count, u
     }
     __syncthreads();
     if (threadIdx.x == 0)
-        for (unsigned w = 1; w < kNormThreads / 64; ++w) {
+        for (unsigned w = 1; w < per; ++w) {
             Acc<P> o;
             o.set(sacc[w]);
             all.join(o);
@@ -380,7 +396,7 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
     }
     Acc<P> all;
     Acc<kPInf> top;
-    block_norm<P, EACH, PEAK>(rec, g.count, n, tile, cold, slots, all, top);
+    block_norm<P, EACH, PEAK>(blockDim.x >> 6, rec, g.count, n, tile, cold, slots, all, top);
     if (threadIdx.x == 0) {
         if (part)
             part[blockIdx.x] = all.value();
@@ -390,7 +406,7 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
             write_norm(P, all.value(), total, norm);
     }
     if (EACH && gridDim.x == 1)  // behind block_norm's barrier, which the slots' writes are ahead of
-        for (uint32_t s = wave_id(); s < g.count; s += kNormThreads / 64)
+        for (uint32_t s = wave_id(); s < g.count; s += blockDim.x >> 6)
             tensor_norm<P, 1>(rec, s, tile, slots, each);
 }
 
@@ -471,7 +487,7 @@ __device__ __forceinline__ void scale_tile(const GradRec *rs, const GradRec *rd,
 {
     const uint64_t hi = min(lo + tile, n);
     const uint32_t s0 = uni32(grad_find(rs, count, lo));
-    if (tile == kLeastTile && grad_many(rs, count, s0, hi)) {
+    if (tile == kLeastTile && grad_many(rs, count, s0, hi, kMany)) {
         const uint32_t s1 = uni32(grad_find(rs, count, hi - 1));
         lane_read(rs, s0, s1, lo, hi, [&](uint32_t i, float x) {
             const uint64_t e = lo + i;
@@ -576,7 +592,7 @@ __global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, Gra
     }
     Acc<P> all;
     Acc<kPInf> top;
-    block_norm<P, false, FLAT>(ss, src.count, n, tile, 0, nullptr, all, top);
+    block_norm<P, false, FLAT>(kNormThreads / 64, ss, src.count, n, tile, 0, nullptr, all, top);
     if (threadIdx.x == 0) {
         const double N = root_of(P, all.value());
         sc = clip_coef(N, max_norm);
@@ -1084,7 +1100,12 @@ static uint32_t tile_of(uint64_t n, uint64_t count, uint32_t most, uint64_t few 
 // about what eight elements do.  Clipping 5000 elements of 3 / 60 / 500 tensors
 // takes 6.3 / 11.6 / 18.3 us in one block and 8.3 / 11.1 / 13.4 us in two
 // launches, 20000 of 3 / 60 tensors 8.8 / 19.2 and 9.5 / 11.1 us.
-static bool one_block(uint64_t n, uint64_t count) { return n + 8 * count <= kOneElems; }
+// Each tensor's own norm: four times that (5000 elements of 300 tensors 23.6 us in
+// one block, 14 in two launches).
+static bool one_block(uint64_t n, uint64_t count, bool each = false)
+{
+    return n + (each ? 32 : 8) * count <= kOneElems;
+}
 static_assert(kOneElems / 8 <= kLdsRecs, "one block's table is in LDS");
 
 // The norm's tile: up to 8 KB of gradients.  Each tensor's own norm takes a
@@ -1094,10 +1115,16 @@ static uint32_t norm_tile(const gc_grads *g, bool each = false)
     return tile_of(g->n, g->count, held_bytes(g) < 3 * g->n ? 2 * kTile : kTile, each ? kFewEach : kFewElems);
 }
 
-static unsigned norm_grid(uint64_t n, uint64_t count, uint32_t tile)
+// Threads a block for `tiles` tiles: a short list is spread over more CUs
+static unsigned norm_threads(uint64_t n, uint64_t count, uint32_t tile, bool each = false)
 {
-    const uint64_t tiles = (n + tile - 1) / tile, per = kNormThreads / 64;
-    return one_block(n, count) ? 1u : (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
+    return !one_block(n, count, each) && n <= (uint64_t)kSpread * tile ? kScaleThreads : kNormThreads;
+}
+
+static unsigned norm_grid(uint64_t n, uint64_t count, uint32_t tile, bool each = false)
+{
+    const uint64_t tiles = (n + tile - 1) / tile, per = norm_threads(n, count, tile, each) / 64;
+    return one_block(n, count, each) ? 1u : (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
 }
 
 // of `of` elements or words that take `bytes`, those ahead of the last kCacheBytes
@@ -1139,7 +1166,7 @@ static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, 
 {
     const GradArg a = arg_of(g);
     const uint32_t tile = norm_tile(g, EACH);
-    const dim3 grid(norm_grid(g->n, g->count, tile)), block(kNormThreads);
+    const dim3 grid(norm_grid(g->n, g->count, tile, EACH)), block(norm_threads(g->n, g->count, tile, EACH));
     char *w = static_cast<char *>(ws);  // null: one block, which leaves nothing there
     double *part = reinterpret_cast<double *>(w);
     uint32_t *peak = w ? reinterpret_cast<uint32_t *>(w + kWsPeak) : nullptr;
@@ -1163,8 +1190,9 @@ static unsigned grid_of(uint64_t tiles, unsigned threads, unsigned most)
 }
 
 // threads a block of the scale: large blocks, and so fewer first steps (the
-// partials, the table), where all tiles are under way at once
-static unsigned scale_threads(uint64_t tiles) { return tiles <= kWaves ? kNormThreads : kScaleThreads; }
+// partials, the table), where most tiles are under way at once; a short list is
+// spread over more CUs
+static unsigned scale_threads(uint64_t tiles) { return tiles > kSpread && tiles <= 2 * kWaves ? kNormThreads : kScaleThreads; }
 
 }  // namespace gc
 
@@ -1261,12 +1289,12 @@ int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, 
     else
         launch_norm<false, false>(grads, p, ~0ull, workspace, total, norm, each, st);
     const uint32_t tile = norm_tile(grads, each != nullptr);
-    const unsigned parts = norm_grid(grads->n, grads->count, tile);
+    const unsigned parts = norm_grid(grads->n, grads->count, tile, each != nullptr);
     if (parts > 1) {
         const char *w = static_cast<const char *>(workspace);
         const dim3 grid(1 + (each ? (unsigned)grads->count : 0u));
         with_p(p, [&](auto P) {
-            hipLaunchKernelGGL(k_grad_finish<P()>, grid, dim3(kNormThreads), 0, st, arg_of(grads), tile,
+            hipLaunchKernelGGL(k_grad_finish<P()>, grid, dim3(each ? kNormThreads : 64), 0, st, arg_of(grads), tile,
                                reinterpret_cast<const double *>(w), parts, reinterpret_cast<const double *>(w + kWsSlots),
                                total, norm, each);
         });

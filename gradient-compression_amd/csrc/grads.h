@@ -85,12 +85,13 @@ __device__ __forceinline__ void grad_walk(const GradRec *rec, uint32_t s, uint64
     }
 }
 
-// Whether [lo, hi), which begins in tensor s, may span more than three tensors.
-// A walk waits for the memory once a piece: a range of many takes its elements
-// lane by lane instead, each lane with the tensors of its own (grad_lane).
-__device__ __forceinline__ bool grad_many(const GradRec *rec, uint32_t count, uint32_t s, uint64_t hi)
+// Whether [lo, hi), which begins in tensor s, spans more than `many` tensors
+// (empty ones count).  A walk waits for the memory once a piece: a range of many
+// takes its elements lane by lane instead, each lane with the tensors of its own
+// (grad_lane).
+__device__ __forceinline__ bool grad_many(const GradRec *rec, uint32_t count, uint32_t s, uint64_t hi, uint32_t many)
 {
-    return uni64(rec[min(s + 3, count)].start) < hi;
+    return uni64(rec[min(s + many, count)].start) < hi;
 }
 
 // the lane's tensor of element e, known to be in s .. last
