@@ -59,10 +59,11 @@ constexpr uint64_t kWaves = 8192;  // resident at once: 256 CUs of 32
 constexpr uint64_t kSpread = 1024;
 
 // Words: one block a CU adds them (128 / 256 / 512 blocks: 33.3 / 30.9 / 32.5 us
-// with the decode, whose every block reads the partials), 4096 decode them
-// (2048 / 4096 / 8192: 285 / 258 / 260 us for 246M elements).
+// with the decode, whose every block reads the partials), four rounds of the
+// blocks that are resident at once decode them (2560 / 4096 / 5120 / 8192: 254 /
+// 259 / 250 / 249 us for 246M bfloat16, 96.4 / 95.3 / 95.1 / 95.2 us for 100M float32).
 constexpr unsigned kLaneGrid = 256;
-constexpr unsigned kDecodeGrid = 4096;
+constexpr unsigned kDecodeGrid = 5120;
 
 // What one block does alone (one_block) and the average sizes below which
 // tensors count as small: for the sums and the scaling of a list, and for
@@ -375,14 +376,14 @@ __device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, uint
         each[s] = (float)root_of(P, t);
 }
 
-// The norm's first pass: one partial a block; a grid of one block finishes the
-// call itself.  A block's tiles are 16 consecutive ones of every gridDim.x * 16,
+// The norm's first pass: one partial a block, or the whole call in one block
+// (alone).  A block's tiles are 16 consecutive ones of every gridDim.x * 16,
 // so the chip reads a few MB of consecutive addresses at any time.  Bound by
 // HBM: 4 GB of float32 in 579 us (6.9 TB/s), 853 MB of bfloat16 in 125 us
 // (6.8 TB/s; 132 us with each tensor's norm); 94 MB of float32 in 17 us, of which
 // 4 us are the launch and the first loads.
 template <int P, bool EACH, bool PEAK, bool LDS>
-__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, uint32_t tile, uint64_t cold,
+__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, uint32_t tile, uint64_t cold, bool alone,
                                                                double *__restrict__ part,
                                                                uint32_t *__restrict__ peak, double *slots,
                                                                double *__restrict__ total, float *__restrict__ norm,
@@ -402,10 +403,10 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
             part[blockIdx.x] = all.value();
         if (PEAK)
             peak[blockIdx.x] = top.m;
-        if (gridDim.x == 1)
+        if (alone)
             write_norm(P, all.value(), total, norm);
     }
-    if (EACH && gridDim.x == 1)  // behind block_norm's barrier, which the slots' writes are ahead of
+    if (EACH && alone)  // behind block_norm's barrier, which the slots' writes are ahead of
         for (uint32_t s = wave_id(); s < g.count; s += blockDim.x >> 6)
             tensor_norm<P, 1>(rec, s, tile, slots, each);
 }
@@ -839,9 +840,11 @@ __device__ __forceinline__ void decode_whole(const DecodeArg &d, const Unit &x, 
     }
 }
 
-// Issue bound until the lookups were shared out: lane l finds plane l0 + l's
-// tensor (at most 32 planes), all at once, and a plane that lies whole in one
-// tensor is written without a test.
+// Issue bound until the lookups were shared out (30.3 us for ResNet50's 23.5M at
+// 4 bits, 28.4 since): lane l finds plane l0 + l's tensor (at most 32 planes),
+// all at once, and a plane that lies whole in one tensor is written without a
+// test.  A range of many tensors is written lane by lane (1000 elements of 480
+// tensors 22 -> 7 us).
 __device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd, uint32_t count, const Unit &x, float k, float c)
 {
     constexpr uint32_t kWords = 256 * kQuads;
@@ -877,7 +880,25 @@ __device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd,
                 decode_whole<_Float16>(d, x, sh, glob<_Float16>(base, lo - start));
             continue;
         }
-        grad_walk(rd, (uint32_t)__builtin_amdgcn_readlane((int)mine, at), lo, hi,
+        const uint32_t s0 = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+        if (grad_many(rd, count, s0, hi, kMany)) {
+            const uint32_t s1 = uni32(grad_find(rd, count, hi - 1));
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                float v[4];
+                decode_quad(d, x.wd[q], sh, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint64_t i = lo + 256 * q + 4 * lane + e;
+                    if (i < hi) {
+                        const uint32_t s = grad_lane(rd, s0, s1, i);
+                        st_any(rd[s].pt, i - rd[s].start, v[e]);
+                    }
+                }
+            }
+            continue;
+        }
+        grad_walk(rd, s0, lo, hi,
                   [&](uint32_t, uint32_t type, uint64_t base, uint64_t tstart, uint64_t pa, uint64_t pb) {
 #pragma unroll
                       for (int q = 0; q < kQuads; ++q) {
@@ -1166,6 +1187,7 @@ static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, 
 {
     const GradArg a = arg_of(g);
     const uint32_t tile = norm_tile(g, EACH);
+    const bool alone = one_block(g->n, g->count, EACH);
     const dim3 grid(norm_grid(g->n, g->count, tile, EACH)), block(norm_threads(g->n, g->count, tile, EACH));
     char *w = static_cast<char *>(ws);  // null: one block, which leaves nothing there
     double *part = reinterpret_cast<double *>(w);
@@ -1173,11 +1195,11 @@ static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, 
     double *slots = w ? reinterpret_cast<double *>(w + kWsSlots) : nullptr;
     with_p(p, [&](auto P) {
         if (g->count <= kLdsRecs)
-            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, tile, cold, part, peak, slots,
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, tile, cold, alone, part, peak, slots,
                                total,
                                norm, each);
         else
-            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, tile, cold, part, peak, slots,
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, tile, cold, alone, part, peak, slots,
                                total,
                                norm, each);
     });
@@ -1290,7 +1312,7 @@ int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, 
         launch_norm<false, false>(grads, p, ~0ull, workspace, total, norm, each, st);
     const uint32_t tile = norm_tile(grads, each != nullptr);
     const unsigned parts = norm_grid(grads->n, grads->count, tile, each != nullptr);
-    if (parts > 1) {
+    if (!one_block(grads->n, grads->count, each != nullptr)) {
         const char *w = static_cast<const char *>(workspace);
         const dim3 grid(1 + (each ? (unsigned)grads->count : 0u));
         with_p(p, [&](auto P) {
