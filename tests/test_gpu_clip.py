@@ -668,3 +668,20 @@ def test_lists_on_another_stream():
             want = res if want is None else want
             del ts, flat
             assert torch.equal(res, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [8_193, 1_100_000, 9_000_001, 30_000_001, 70_000_003])
+def test_each_norm_over_the_tile_sizes(n, dtype):
+    """Ones: every sum is a whole number, whatever tile and slots a list of n elements is given."""
+    ts = [torch.ones(n, dtype=dtype, device=DEV), torch.ones(5, dtype=dtype, device=DEV), torch.ones(n // 3, dtype=dtype, device=DEV)]
+    m = [t.numel() for t in ts]
+    total, each = gcodec.grad_norm(ts, 1, per_tensor=True)
+    assert float(total) == float(np.float32(sum(m))) and each.tolist() == [float(np.float32(k)) for k in m]
+    total, each = gcodec.grad_norm(ts, 2, per_tensor=True)
+    assert float(total) == float(np.float32(math.sqrt(sum(m))))
+    assert each.tolist() == [float(np.float32(math.sqrt(k))) for k in m]
+    for t in ts:
+        t[-1] = 3.0
+    total, each = gcodec.grad_norm(ts, INF, per_tensor=True)
+    assert float(total) == 3.0 and each.tolist() == [3.0] * 3
