@@ -205,15 +205,14 @@ __device__ __forceinline__ void lane_read(const GradRec *rec, uint32_t s0, uint3
             f(u * 64 + lane_id(), x[u]);
 }
 
-// The share of a block of `per` waves of the sum of |x|^p and (PEAK) of max |x|, valid in thread 0.
+// The share of a block of `per` waves of the sum of |x|^p and (PEAK) of max |x|,
+// valid in thread 0; elements ahead of `cold` are read past the cache.
 // EACH: also the sum of every piece, at slot (tile + tensor): along the flat
 // sequence each next piece has the next tile or the next tensor, so a tensor's
 // pieces have consecutive slots of their own.
 template <int P, bool EACH, bool PEAK>
 __device__ __forceinline__ void block_norm(uint32_t per, const GradRec *rec, uint32_t count, uint64_t n, uint32_t tile,
-                                           uint64_t cold,
-                                           double *__restrict__ slots,
-                                           Acc<P> &all, Acc<kPInf> &top)
+                                           uint64_t cold, double *__restrict__ slots, Acc<P> &all, Acc<kPInf> &top)
 {
     __shared__ double sacc[kNormThreads / 64];
     __shared__ uint32_t smax[kNormThreads / 64];
@@ -383,8 +382,8 @@ __device__ __forceinline__ void tensor_norm(const GradRec *rec, uint32_t s, uint
 // (6.8 TB/s; 132 us with each tensor's norm); 94 MB of float32 in 17 us, of which
 // 4 us are the launch and the first loads.
 template <int P, bool EACH, bool PEAK, bool LDS>
-__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, uint32_t tile, uint64_t cold, bool alone,
-                                                               double *__restrict__ part,
+__global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64_t n, uint32_t tile, uint64_t cold,
+                                                               bool alone, double *__restrict__ part,
                                                                uint32_t *__restrict__ peak, double *slots,
                                                                double *__restrict__ total, float *__restrict__ norm,
                                                                float *__restrict__ each)
@@ -412,11 +411,11 @@ __global__ __launch_bounds__(kNormThreads, 8) void k_grad_norm(GradArg g, uint64
 }
 
 // The norm's second pass, over the partials.  Block 0: the total and N; block
-// 1 + s: the norm of tensor s.  Latency: 2 us queued behind the first pass; 6 us
-// with each norm, where the largest tensor has 16,000 slots.
+// 1 + s: the norm of tensor s.  Latency: 4 us for 512 partials, 6.5 us with each
+// norm where the largest tensor has 16,000 slots.
 template <int P>
-__global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, uint32_t tile, const double *__restrict__ part, uint32_t parts,
-                                                              const double *__restrict__ slots,
+__global__ __launch_bounds__(kNormThreads) void k_grad_finish(GradArg g, uint32_t tile, const double *__restrict__ part,
+                                                              uint32_t parts, const double *__restrict__ slots,
                                                               double *__restrict__ total, float *__restrict__ norm,
                                                               float *__restrict__ each)
 {
@@ -480,8 +479,8 @@ __device__ __forceinline__ void wave_scale_to(uint32_t td, Glob<const TS> x, uin
         wave_scale<TS, _Float16, NT>(x, glob<_Float16>(base, off), cnt, c);
 }
 
-// The tile from element lo on of y = RN(x c), from the tensors of src into those of dst (the same
-// sizes), or (FLAT) end to end into float32
+// The tile from element lo on of y = RN(x c), from the tensors of src into those
+// of dst (the same sizes), or (FLAT) end to end into float32
 template <bool FLAT, bool NT>
 __device__ __forceinline__ void scale_tile(const GradRec *rs, const GradRec *rd, uint32_t count, float *flat, uint64_t n,
                                            uint64_t lo, uint32_t tile, float c)
@@ -523,9 +522,9 @@ __device__ __forceinline__ void scale_tile(const GradRec *rs, const GradRec *rd,
 // bucket).  Bound by HBM: 1.7 GB in 248 us (6.9 TB/s, a part from the cache);
 // 118 MB of 14.7M float32 in 22 us, 188 MB of 23.5M into a bucket in 31 us.
 template <bool FLAT, bool LDS>
-__global__ __launch_bounds__(kNormThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n, uint32_t tile,
-                                                              uint64_t cold, int p,
-                                                              double max_norm, const double *__restrict__ part,
+__global__ __launch_bounds__(kNormThreads) void k_grad_scale(GradArg src, GradArg dst, float *flat, uint64_t n,
+                                                              uint32_t tile, uint64_t cold, int p, double max_norm,
+                                                              const double *__restrict__ part,
                                                               uint32_t parts, const uint32_t *__restrict__ peaks,
                                                               bool in_place, float *__restrict__ norm,
                                                               float *__restrict__ peak)
@@ -579,8 +578,7 @@ __global__ __launch_bounds__(kNormThreads) void k_grad_scale(GradArg src, GradAr
 template <int P, bool FLAT>
 __global__ __launch_bounds__(kNormThreads) void k_grad_clip_one(GradArg src, GradArg dst, float *flat, uint64_t n,
                                                                 uint32_t tile, double max_norm, bool in_place,
-                                                                float *__restrict__ norm,
-                                                                float *__restrict__ peak)
+                                                                float *__restrict__ norm, float *__restrict__ peak)
 {
     __shared__ GradRec ss[kLdsRecs + 1];
     __shared__ GradRec sd[FLAT ? 1 : kLdsRecs + 1];
@@ -673,8 +671,8 @@ __device__ __forceinline__ double lanes_root(const LaneArg &a, float k, bool exa
 
 // four words' lanes l0 <= l < l1 at flat elements l M + i .. + 3; CHECK: those below n
 template <int P, bool CHECK>
-__device__ __forceinline__ uint32_t quad_sum(const LaneArg &a, uint4 wd, uint64_t i, uint32_t l0, uint32_t l1, uint32_t mask,
-                                             uint32_t sum)
+__device__ __forceinline__ uint32_t quad_sum(const LaneArg &a, uint4 wd, uint64_t i, uint32_t l0, uint32_t l1,
+                                             uint32_t mask, uint32_t sum)
 {
     for (uint32_t l = l0; l < l1; ++l) {
         const uint32_t we[4] = {wd.x, wd.y, wd.z, wd.w};
@@ -772,7 +770,8 @@ __global__ __launch_bounds__(kNormThreads) void k_lane_norm(LaneArg a, uint64_t 
 // the lane's quad v of flat elements i .. i + 3, those inside [a, b), to the
 // tensor at base whose first element is start
 template <class T>
-__device__ __forceinline__ void store_quad(uint64_t base, uint64_t start, uint64_t a, uint64_t b, uint64_t i, const float (&v)[4])
+__device__ __forceinline__ void store_quad(uint64_t base, uint64_t start, uint64_t a, uint64_t b, uint64_t i,
+                                           const float (&v)[4])
 {
     const Glob<T> y = glob<T>(base, 0);
     if (i >= a && i + 4 <= b) {
@@ -845,7 +844,8 @@ __device__ __forceinline__ void decode_whole(const DecodeArg &d, const Unit &x, 
 // all at once, and a plane that lies whole in one tensor is written without a
 // test.  A range of many tensors is written lane by lane (1000 elements of 480
 // tensors 22 -> 7 us).
-__device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd, uint32_t count, const Unit &x, float k, float c)
+__device__ __forceinline__ void decode_unit(const LaneArg &a, const GradRec *rd, uint32_t count, const Unit &x, float k,
+                                            float c)
 {
     constexpr uint32_t kWords = 256 * kQuads;
     const DecodeArg d{k, a.alpha, c, a.sub, a.w >= 32 ? 0xffffffffu : (1u << a.w) - 1u};
@@ -1156,7 +1156,9 @@ static unsigned norm_threads(uint64_t n, uint64_t count, uint32_t tile, bool eac
 static unsigned norm_grid(uint64_t n, uint64_t count, uint32_t tile, bool each = false)
 {
     const uint64_t tiles = (n + tile - 1) / tile, per = norm_threads(n, count, tile, each) / 64;
-    return one_block(n, count, each) ? 1u : (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
+    if (one_block(n, count, each))
+        return 1;
+    return (unsigned)std::min<uint64_t>(std::max<uint64_t>((tiles + per - 1) / per, 1), kNormGrid);
 }
 
 // of `of` elements or words that take `bytes`, those ahead of the last kCacheBytes
@@ -1206,13 +1208,11 @@ static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, 
     double *slots = w ? reinterpret_cast<double *>(w + kWsSlots) : nullptr;
     with_p(p, [&](auto P) {
         if (g->count <= kLdsRecs)
-            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, tile, cold, alone, part, peak, slots,
-                               total,
-                               norm, each);
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, true>), grid, block, 0, st, a, g->n, tile, cold, alone,
+                               part, peak, slots, total, norm, each);
         else
-            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, tile, cold, alone, part, peak, slots,
-                               total,
-                               norm, each);
+            hipLaunchKernelGGL((k_grad_norm<P(), EACH, PEAK, false>), grid, block, 0, st, a, g->n, tile, cold, alone,
+                               part, peak, slots, total, norm, each);
     });
 }
 
@@ -1225,7 +1225,10 @@ static unsigned grid_of(uint64_t tiles, unsigned threads, unsigned most)
 // threads a block of the scale: large blocks, and so fewer first steps (the
 // partials, the table), where most tiles are under way at once; a short list is
 // spread over more CUs
-static unsigned scale_threads(uint64_t tiles) { return tiles > kSpread && tiles <= 2 * kWaves ? kNormThreads : kScaleThreads; }
+static unsigned scale_threads(uint64_t tiles)
+{
+    return tiles > kSpread && tiles <= 2 * kWaves ? kNormThreads : kScaleThreads;
+}
 
 }  // namespace gc
 
@@ -1345,8 +1348,8 @@ int gc_grad_norm_root(const double *total, uint32_t p, float *norm, gc_stream_t 
         return rc;
     GC_REQUIRE(total && norm, "%s: null pointer", what);
     with_p(p, [&](auto P) {
-        hipLaunchKernelGGL(k_grad_finish<P()>, dim3(1), dim3(64), 0, as_stream(stream), GradArg{nullptr, 0}, kTile, total, 1u,
-                           nullptr, nullptr, norm, nullptr);
+        hipLaunchKernelGGL(k_grad_finish<P()>, dim3(1), dim3(64), 0, as_stream(stream), GradArg{nullptr, 0}, kTile,
+                           total, 1u, nullptr, nullptr, norm, nullptr);
     });
     return launch_status(what);
 }
@@ -1363,7 +1366,8 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
                (unsigned long long)dst->count);
     bool same = true;
     for (uint64_t s = 0; s <= src->count; ++s) {
-        GC_REQUIRE(src->host_rec[2 * s + 1] == dst->host_rec[2 * s + 1], "%s: the two lists differ in tensor sizes", what);
+        GC_REQUIRE(src->host_rec[2 * s + 1] == dst->host_rec[2 * s + 1],
+                   "%s: the two lists differ in tensor sizes", what);
         same &= src->host_rec[2 * s] == dst->host_rec[2 * s];
     }
     if (!same && (rc = check_apart(src, dst, what)))
@@ -1371,10 +1375,11 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
     if (!total && (rc = check_workspace(src, false, workspace, what)))
         return rc;
     hipStream_t st = as_stream(stream);
+    const uint32_t tile = tile_of(src->n, src->count, kTile);
     if (!total && one_block(src->n, src->count)) {
         with_p(p, [&](auto P) {
-            hipLaunchKernelGGL((k_grad_clip_one<P(), false>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), arg_of(dst),
-                               nullptr, src->n, tile_of(src->n, src->count, kTile), max_norm, same, norm, nullptr);
+            hipLaunchKernelGGL((k_grad_clip_one<P(), false>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src),
+                               arg_of(dst), nullptr, src->n, tile, max_norm, same, norm, nullptr);
         });
         return launch_status(what);
     }
@@ -1382,16 +1387,15 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
         launch_norm<false, false>(src, p, cold_elems(src), workspace, nullptr, nullptr, nullptr, st);
     const double *part = total ? total : static_cast<const double *>(workspace);
     const unsigned parts = total ? 1u : norm_grid(src->n, src->count, norm_tile(src));
-    const uint32_t tile = tile_of(src->n, src->count, kTile);
     const uint64_t tiles = (src->n + tile - 1) / tile;
     const unsigned threads = scale_threads(tiles), grid = grid_of(tiles, threads, kScaleGrid);
     const GradArg a = arg_of(src), b = arg_of(dst);
     if (src->count <= kLdsRecs)
-        hipLaunchKernelGGL((k_grad_scale<false, true>), dim3(grid), dim3(threads), 0, st, a, b, nullptr, src->n, tile, cold_elems(src),
-                           (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
+        hipLaunchKernelGGL((k_grad_scale<false, true>), dim3(grid), dim3(threads), 0, st, a, b, nullptr, src->n, tile,
+                           cold_elems(src), (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
     else
-        hipLaunchKernelGGL((k_grad_scale<false, false>), dim3(grid), dim3(threads), 0, st, a, b, nullptr, src->n, tile, cold_elems(src),
-                           (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
+        hipLaunchKernelGGL((k_grad_scale<false, false>), dim3(grid), dim3(threads), 0, st, a, b, nullptr, src->n, tile,
+                           cold_elems(src), (int)p, max_norm, part, parts, nullptr, same, norm, nullptr);
     return launch_status(what);
 }
 
@@ -1413,27 +1417,28 @@ int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double ma
                    (unsigned long long)s);
     }
     hipStream_t st = as_stream(stream);
+    const uint32_t tile = tile_of(src->n, src->count, kTile);
     if (one_block(src->n, src->count)) {
         with_p(p, [&](auto P) {
-            hipLaunchKernelGGL((k_grad_clip_one<P(), true>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src), GradArg{}, flat,
-                               src->n, tile_of(src->n, src->count, kTile), max_norm, false, norm, peak);
+            hipLaunchKernelGGL((k_grad_clip_one<P(), true>), dim3(1), dim3(kNormThreads), 0, st, arg_of(src),
+                               GradArg{}, flat, src->n, tile, max_norm, false, norm, peak);
         });
         return launch_status(what);
     }
     launch_norm<false, true>(src, p, cold_elems(src), workspace, nullptr, nullptr, nullptr, st);
     const char *w = static_cast<const char *>(workspace);
-    const uint32_t tile = tile_of(src->n, src->count, kTile);
     const uint64_t tiles = (src->n + tile - 1) / tile;
-    const unsigned threads = scale_threads(tiles), grid = grid_of(tiles, threads, kScaleGrid), parts = norm_grid(src->n, src->count, norm_tile(src));
+    const unsigned threads = scale_threads(tiles), grid = grid_of(tiles, threads, kScaleGrid);
+    const unsigned parts = norm_grid(src->n, src->count, norm_tile(src));
     const GradArg a = arg_of(src);
     const double *part = reinterpret_cast<const double *>(w);
     const uint32_t *peaks = reinterpret_cast<const uint32_t *>(w + kWsPeak);
     if (src->count <= kLdsRecs)
-        hipLaunchKernelGGL((k_grad_scale<true, true>), dim3(grid), dim3(threads), 0, st, a, GradArg{}, flat, src->n, tile, cold_elems(src),
-                           (int)p, max_norm, part, parts, peaks, false, norm, peak);
+        hipLaunchKernelGGL((k_grad_scale<true, true>), dim3(grid), dim3(threads), 0, st, a, GradArg{}, flat, src->n, tile,
+                           cold_elems(src), (int)p, max_norm, part, parts, peaks, false, norm, peak);
     else
-        hipLaunchKernelGGL((k_grad_scale<true, false>), dim3(grid), dim3(threads), 0, st, a, GradArg{}, flat, src->n, tile, cold_elems(src),
-                           (int)p, max_norm, part, parts, peaks, false, norm, peak);
+        hipLaunchKernelGGL((k_grad_scale<true, false>), dim3(grid), dim3(threads), 0, st, a, GradArg{}, flat, src->n,
+                           tile, cold_elems(src), (int)p, max_norm, part, parts, peaks, false, norm, peak);
     return launch_status(what);
 }
 
