@@ -1027,11 +1027,21 @@ static int check_output(const gc_grads *g, const char *what)
     return GC_OK;
 }
 
-// whether [lo, hi) meets a tensor of the (disjoint) table; *at the first one's index
+// whether [lo, hi) meets a tensor of the table; *at the first one's index
 static bool meets(const gc_grads *g, Span x, uint64_t *at)
 {
     if (x.lo >= x.hi)
         return false;
+    if (g->flags & GC_GRADS_OVERLAP) {  // a later tensor may end ahead of an earlier one
+        for (uint64_t s = 0; s < g->count; ++s) {
+            const Span y = span_of(g, s);
+            if (y.lo < y.hi && y.lo < x.hi && x.lo < y.hi) {
+                *at = s;
+                return true;
+            }
+        }
+        return false;
+    }
     uint64_t a = 0, b = g->count;  // order[]: non-empty tensors by address, then the empty ones
     while (a < b) {
         const uint64_t m = (a + b) / 2;
@@ -1072,6 +1082,38 @@ static int check_apart(const gc_grads *src, const gc_grads *dst, const char *wha
             GC_REQUIRE(s == d && src->host_rec[2 * s] == dst->host_rec[2 * s],
                        "%s: input tensor %u shares memory with output tensor %u", what, s, d);
         }
+    }
+    return GC_OK;
+}
+
+// Memory that a call uses beside its tensors
+struct Side {
+    const char *name;
+    const void *at;  // null: not used
+    uint64_t bytes;
+    bool written;
+};
+
+// Blocks that are done write norms, totals and the output while others still read:
+// what a call writes shares memory with nothing else that it uses.
+template <size_t N>
+static int check_sides(const Side (&side)[N], const gc_grads *src, const gc_grads *dst, const char *what)
+{
+    for (size_t i = 0; i < N; ++i) {
+        const uint64_t lo = reinterpret_cast<uint64_t>(side[i].at);
+        const Span x{lo, side[i].at ? lo + side[i].bytes : lo};
+        if (x.lo == x.hi)
+            continue;
+        for (size_t j = i + 1; j < N; ++j) {
+            const uint64_t at = reinterpret_cast<uint64_t>(side[j].at);
+            GC_REQUIRE(!(side[i].written || side[j].written) || !at || at >= x.hi || at + side[j].bytes <= x.lo,
+                       "%s: %s and %s share memory", what, side[i].name, side[j].name);
+        }
+        uint64_t at = 0;
+        GC_REQUIRE(!(src && side[i].written && meets(src, x, &at)), "%s: %s shares memory with input tensor %llu", what,
+                   side[i].name, (unsigned long long)at);
+        GC_REQUIRE(!(dst && meets(dst, x, &at)), "%s: %s shares memory with output tensor %llu", what, side[i].name,
+                   (unsigned long long)at);
     }
     return GC_OK;
 }
@@ -1180,6 +1222,11 @@ static int check_workspace(const gc_grads *g, bool each, const void *workspace, 
     GC_REQUIRE(workspace || gc_grad_workspace_size(g->n, g->count, each) == 0, "%s: null workspace", what);
     GC_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: misaligned workspace", what);
     return GC_OK;
+}
+
+static Side workspace_side(const gc_grads *g, bool each, const void *workspace)
+{
+    return {"the workspace", workspace, gc_grad_workspace_size(g->n, g->count, each), true};
 }
 
 // f(p as a constant)
@@ -1321,6 +1368,10 @@ int gc_grad_norm(const gc_grads *grads, uint32_t p, double *total, float *norm, 
         return rc;
     if ((rc = check_workspace(grads, each != nullptr, workspace, what)))
         return rc;
+    const Side side[] = {{"total", total, 8, true}, {"norm", norm, 4, true}, {"each", each, 4 * grads->count, true},
+                         workspace_side(grads, each != nullptr, workspace)};
+    if ((rc = check_sides(side, grads, nullptr, what)))
+        return rc;
     hipStream_t st = as_stream(stream);
     if (each)
         launch_norm<true, false>(grads, p, ~0ull, workspace, total, norm, each, st);
@@ -1374,6 +1425,10 @@ int gc_grad_clip(const gc_grads *src, const gc_grads *dst, uint32_t p, double ma
         return rc;
     if (!total && (rc = check_workspace(src, false, workspace, what)))
         return rc;
+    const Side side[] = {{"norm", norm, 4, true}, {"total", total, 8, false},
+                         workspace_side(src, false, total ? nullptr : workspace)};
+    if ((rc = check_sides(side, src, dst, what)))
+        return rc;
     hipStream_t st = as_stream(stream);
     const uint32_t tile = tile_of(src->n, src->count, kTile);
     if (!total && one_block(src->n, src->count)) {
@@ -1410,12 +1465,10 @@ int gc_grad_flatten_clip(const gc_grads *src, float *flat, uint32_t p, double ma
                "%s: null or misaligned output", what);
     if ((rc = check_workspace(src, false, workspace, what)))
         return rc;
-    const uint64_t lo = reinterpret_cast<uint64_t>(flat), hi = lo + 4 * src->n;
-    for (uint64_t s = 0; s < src->count; ++s) {
-        const Span x = span_of(src, s);
-        GC_REQUIRE(x.lo >= x.hi || x.hi <= lo || x.lo >= hi, "%s: input tensor %llu lies in the flat bucket", what,
-                   (unsigned long long)s);
-    }
+    const Side side[] = {{"the flat bucket", flat, 4 * src->n, true}, {"peak", peak, 4, true}, {"norm", norm, 4, true},
+                         workspace_side(src, false, workspace)};
+    if ((rc = check_sides(side, src, nullptr, what)))
+        return rc;
     hipStream_t st = as_stream(stream);
     const uint32_t tile = tile_of(src->n, src->count, kTile);
     if (one_block(src->n, src->count)) {
@@ -1459,10 +1512,10 @@ int gc_qsgd_decode_clip(const uint32_t *words, uint64_t n, const float *norm, ui
     GC_REQUIRE(aligned16(words), "%s: words must be 16-byte aligned", what);
     if ((rc = check_workspace(dst, false, workspace, what)))
         return rc;
-    uint64_t at = 0;
-    const uint64_t w0 = reinterpret_cast<uint64_t>(words), m0 = reinterpret_cast<uint64_t>(norm);
-    GC_REQUIRE(!meets(dst, {w0, w0 + 4 * lanes->plane_words}, &at) && !meets(dst, {m0, m0 + 4}, &at),
-               "%s: output tensor %llu shares memory with the words or the norm", what, (unsigned long long)at);
+    const Side side[] = {{"the words", words, 4 * lanes->plane_words, false}, {"norm", norm, 4, false},
+                         {"total_norm", total_norm, 4, true}, workspace_side(dst, false, workspace)};
+    if ((rc = check_sides(side, nullptr, dst, what)))
+        return rc;
     hipStream_t st = as_stream(stream);
     const LaneArg a{words, n, lanes->plane_words, norm, (float)s, alpha, (int32_t)(lanes->world * s), lanes->bits,
                     lanes->per_word, lanes->world * s, cold_part(lanes->plane_words, 4 * lanes->plane_words),

@@ -320,7 +320,9 @@ int gc_qsgd_decode_segments(const uint32_t *words, uint64_t n, const float *norm
  * Sums are 64-bit floating point in an order fixed by n and the tensor list, so
  * results repeat bit for bit.  No entry point below uses atomics, keeps state or
  * needs a zeroed workspace: the workspace (gc_grad_workspace_size bytes, 8-byte
- * aligned) belongs to the call until its kernels have run.
+ * aligned) belongs to the call until its kernels have run.  What a call writes beside
+ * the tensors (norms, totals, the max-norm, the bucket, the workspace) shares memory
+ * with nothing else that the call uses.
  * Replaces, for a list of gradients, what a trainer does between the reducers
  * (reducer.py:498-554) and the optimizer step (trainer.py:183-196). */
 #define GC_F32 16u

@@ -142,6 +142,51 @@ def test_decode_refuses():
     assert call(twice) == _lib.GC_EINVAL and "share memory" in err()
 
 
+def test_what_a_call_writes_beside_the_tensors_stands_alone():
+    """Blocks that are done write the norm while others still read: it shares memory with nothing the call uses."""
+    lib = _lib.load()
+    n = 20_000  # two launches
+    a, b = Table([n, 8], [0x40000, 0x2000], [F32, F16]), Table([n, 8], [0x80000, 0x3000], [F32, F16])
+    ln = _lib.gc_lanes()
+    assert lib.gc_qsgd_layout(n + 8, 4, 1, C.byref(ln)) == 0
+    words, scale = 0x300000, 0x9000
+
+    def decode(out, norm=scale, ws=WS):
+        return lib.gc_qsgd_decode_clip(words, n + 8, norm, 4, C.byref(ln), 1.0, b.ref, 2, 1.0, out, ws, None)
+
+    for rc, msg in [
+        (lambda: decode(scale), "share memory"),                          # the scale that every block reads
+        (lambda: decode(words + 4 * ln.plane_words - 4), "share memory"),  # the last word
+        (lambda: decode(0x80000 + 4 * n - 4), "output tensor 0"),
+        (lambda: decode(0x3000), "output tensor 1"),
+        (lambda: decode(WS), "share memory"),
+        (lambda: decode(NORM, norm=WS + 8), "share memory"),
+        (lambda: decode(NORM, ws=words), "share memory"),
+        (lambda: decode(NORM, ws=0x80000), "output tensor 0"),
+        (lambda: clip_call(a, b, norm=0x40000), "input tensor 0"),
+        (lambda: clip_call(a, b, norm=0x2008), "input tensor 1"),
+        (lambda: clip_call(a, b, norm=0x80004), "output tensor 0"),
+        (lambda: clip_call(a, a, norm=0x40004), "tensor 0"),
+        (lambda: clip_call(a, b, norm=WS + 16), "share memory"),
+        (lambda: clip_call(a, b, total=NORM, norm=NORM + 4), "share memory"),
+        (lambda: clip_call(a, b, total=0x80000), "output tensor 0"),
+        (lambda: clip_call(a, b, ws=0x40000), "input tensor 0"),
+        (lambda: lib.gc_grad_flatten_clip(a.ref, 0x400000, 2, 1.0, NORM, NORM, WS, None), "share memory"),
+        (lambda: lib.gc_grad_flatten_clip(a.ref, 0x400000, 2, 1.0, 0x400010, NORM, WS, None), "share memory"),
+        (lambda: lib.gc_grad_flatten_clip(a.ref, 0x400000, 2, 1.0, NORM, 0x40010, WS, None), "input tensor 0"),
+        (lambda: lib.gc_grad_flatten_clip(a.ref, 0x400000, 2, 1.0, NORM, NORM + 4, 0x400000, None), "share memory"),
+        (lambda: lib.gc_grad_norm(a.ref, 2, NORM, NORM, None, WS, None), "share memory"),
+        (lambda: lib.gc_grad_norm(a.ref, 2, None, NORM, NORM - 4, WS, None), "share memory"),
+        (lambda: lib.gc_grad_norm(a.ref, 2, None, NORM, WS + 6144, WS, None), "share memory"),
+        (lambda: lib.gc_grad_norm(a.ref, 2, None, 0x40000, None, WS, None), "input tensor 0"),
+    ]:
+        assert rc() == _lib.GC_EINVAL and msg in err(), err()
+    twice = Table([n, n, 4], [0x40000, 0x40100, 0x1000], [F32, F32, F32])  # a list that is only read may overlap itself
+    for at, tensor in ((0x1008, 2), (0x40000, 0), (0x40100 + 4 * n - 4, 1)):
+        assert lib.gc_grad_norm(twice.ref, 2, None, at, None, WS, None) == _lib.GC_EINVAL
+        assert f"input tensor {tensor}" in err(), err()
+
+
 def test_python_refusals():
     x = torch.ones(4)
     with pytest.raises(_lib.GCodecError, match="no CPU fallback"):
