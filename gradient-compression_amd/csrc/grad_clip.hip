@@ -1249,7 +1249,7 @@ static void launch_norm(const gc_grads *g, uint32_t p, uint64_t cold, void *ws, 
     const uint32_t tile = norm_tile(g, EACH);
     const bool alone = one_block(g->n, g->count, EACH);
     const dim3 grid(norm_grid(g->n, g->count, tile, EACH)), block(norm_threads(g->n, g->count, tile, EACH));
-    char *w = static_cast<char *>(ws);  // null: one block, which leaves nothing there
+    char *w = alone && !EACH ? nullptr : static_cast<char *>(ws);  // one block leaves no partials
     double *part = reinterpret_cast<double *>(w);
     uint32_t *peak = w ? reinterpret_cast<uint32_t *>(w + kWsPeak) : nullptr;
     double *slots = w ? reinterpret_cast<double *>(w + kWsSlots) : nullptr;

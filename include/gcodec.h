@@ -344,7 +344,7 @@ int gc_grads_plan(const uint64_t *sizes, const void *const *ptrs, const uint32_t
                   uint64_t *rec_host, uint32_t *order, gc_grads *out);
 int gc_grads_fill(const gc_grads *grads, uint64_t *rec, gc_stream_t stream);
 /* each != 0: with room for the per-tensor norms of gc_grad_norm.  0 for the
- * shortest lists, whose calls take a NULL workspace */
+ * shortest lists, whose calls touch no workspace and take a NULL one */
 size_t gc_grad_workspace_size(uint64_t n, uint64_t count, int each);
 /* *norm = N; *total = sum |x|^p (max |x|) in 64 bits, what ranks that hold different
  * shards add up (take the maximum of); each[count] = the tensors' own norms.  Any of

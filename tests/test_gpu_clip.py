@@ -685,3 +685,26 @@ def test_each_norm_over_the_tile_sizes(n, dtype):
         t[-1] = 3.0
     total, each = gcodec.grad_norm(ts, INF, per_tensor=True)
     assert float(total) == 3.0 and each.tolist() == [3.0] * 3
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+def test_short_lists_touch_no_workspace(p):
+    """gc_grad_workspace_size is 0 for them: a pointer that is passed all the same is left alone."""
+    from gcodec import _lib
+
+    lib = _lib.load()
+    ts = views(carve([1000, 3], [F32, BF16], seed=171))
+    g = gcodec.Grads(ts)
+    assert lib.gc_grad_workspace_size(g.n, g.count, 0) == 0
+    ws, norm = torch.full((64,), 7, dtype=torch.int64, device=DEV), torch.zeros((), device=DEV)
+    code = _lib.GC_NORM_INF if p == INF else p
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.gc_grad_norm(g._ref, code, None, norm.data_ptr(), None, ws.data_ptr(), st) == 0
+    close_norm(norm, norm64(f64(ts), p))
+    outs = [torch.empty_like(t) for t in ts]
+    o = gcodec.Grads(outs)
+    assert lib.gc_grad_clip(g._ref, o._ref, code, 0.5, None, norm.data_ptr(), ws.data_ptr(), st) == 0
+    flat, peak = torch.empty(g.n, device=DEV), torch.zeros(1, device=DEV)
+    assert lib.gc_grad_flatten_clip(g._ref, flat.data_ptr(), code, 0.5, peak.data_ptr(), norm.data_ptr(),
+                                    ws.data_ptr(), st) == 0
+    assert bool((ws == 7).all())
