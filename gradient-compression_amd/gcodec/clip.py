@@ -94,7 +94,9 @@ class Grads:
     It keeps the tensors' memory alive, not their shapes or later replacements:
     a gradient that is replaced by another tensor needs another table, and a
     storage that is resized under a table must not be used through it.  A
-    captured call needs its table for as long as the graph is replayed."""
+    captured call needs its table for as long as the graph is replayed.  A
+    write through a table counts as an in-place change of the tensors it was
+    made of, as a write to a list does."""
 
     def __init__(self, tensors):
         tensors = list(tensors)
@@ -106,7 +108,7 @@ class Grads:
         self._rec = rec.to(self.device)  # complete when this returns, whatever stream reads it
         self._home = _raw_stream(self.device.index)
         self.struct.rec = self._rec.data_ptr()
-        self._keep = [t.untyped_storage() for t in tensors]
+        self._tensors = [t.detach() for t in tensors]  # their memory and their version counters
 
     @classmethod
     def _of_call(cls, tensors, of_grads=False, ordered=True):
@@ -115,6 +117,7 @@ class Grads:
         self = cls.__new__(cls)
         if not self._build(tensors, of_grads, ordered):
             return None
+        self._tensors = tensors
         self._rec = torch.empty(len(self._host) // 8, dtype=torch.int64, device=self.device)
         self._home = None
         self.struct.rec = rec = self._rec.data_ptr()
@@ -126,6 +129,7 @@ class Grads:
         lib = _lib.load()
         self.struct = _lib.gc_grads()
         self._ref = C.byref(self.struct)
+        self._of_grads = of_grads
         try:
             got = _lib.tensor_list().gather(tensors, of_grads, ordered, C.cast(lib.gc_grads_plan, C.c_void_p).value,
                                             C.addressof(self.struct))
@@ -153,6 +157,10 @@ class Grads:
                 self._rec.record_stream(torch.cuda.current_stream(self.device))
         return self._ref
 
+    def _written(self):
+        """Tells autograd of a write to the tensors, once the launch is made."""
+        _lib.tensor_list().written(self._tensors, self._of_grads)
+
     def _workspace(self, each: bool = False):
         """A call's workspace, or None where it needs none."""
         size = _lib.load().gc_grad_workspace_size(self.n, self.count, 1) if each else self._ws
@@ -162,8 +170,8 @@ class Grads:
         return torch.empty((), dtype=dtype, device=self.device)
 
 
-def _table(grads, ordered=True, written=False) -> Grads:
-    """The table of a list (written: whose tensors this call writes; autograd is told)."""
+def _table(grads, ordered=True) -> Grads:
+    """The table of a list."""
     if isinstance(grads, Grads):
         return grads
     if isinstance(grads, torch.Tensor):
@@ -173,8 +181,6 @@ def _table(grads, ordered=True, written=False) -> Grads:
     g = Grads._of_call(grads, False, ordered)
     if g is None:
         _refuse("Grads: empty tensor list")
-    if written:
-        _lib.tensor_list().written(grads, False)
     return g
 
 
@@ -237,6 +243,7 @@ def _clip(src: Grads, dst: Grads, max_norm: float, code: int, error_if_nonfinite
     ws = src._workspace()
     _call("gc_grad_clip", src.device, src._use(), dst._use(), code, max_norm,
           _at(total), norm.data_ptr(), _at(ws))
+    dst._written()
     return norm
 
 
@@ -246,8 +253,8 @@ def clip_grads(grads, out, max_norm: float, norm_type: float = 2.0, error_if_non
     tensor may be clipped onto itself; apart from that the tensors of `out`
     share no memory with each other or with `grads`."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
-    src = _table(grads, written=out is grads)
-    dst = src if out is grads else _table(out, written=True)
+    src = _table(grads)
+    dst = src if out is grads else _table(out)
     return _clip(src, dst, max_norm, code, error_if_nonfinite, group, "clip_grads")
 
 
@@ -269,9 +276,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         if error_if_nonfinite:
             _finite(norm, "clip_grad_norm_")
         return norm
-    norm = _clip(src, src, max_norm, code, error_if_nonfinite, group, "clip_grad_norm_")
-    _lib.tensor_list().written(parameters, True)
-    return norm
+    return _clip(src, src, max_norm, code, error_if_nonfinite, group, "clip_grad_norm_")
 
 
 def flatten_clip(grads, max_norm: float, norm_type: float = 2.0, flat=None):
@@ -280,7 +285,8 @@ def flatten_clip(grads, max_norm: float, norm_type: float = 2.0, flat=None):
     by), and the gradients' norm before clipping."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     g = _table(grads)
-    if flat is None:
+    given = flat is not None
+    if not given:
         flat = torch.empty(g.n, dtype=torch.float32, device=g.device)
     elif flat.device != g.device or flat.dtype != torch.float32 or flat.numel() != g.n or not flat.is_contiguous():
         _refuse(f"flatten_clip: flat must be contiguous float32, {g.n} elements on {g.device}")
@@ -289,6 +295,8 @@ def flatten_clip(grads, max_norm: float, norm_type: float = 2.0, flat=None):
     ws = g._workspace()
     _call("gc_grad_flatten_clip", g.device, g._use(), flat.data_ptr(), code, max_norm, peak.data_ptr(), norm.data_ptr(),
           _at(ws))
+    if given:
+        _lib.tensor_list().written([flat], False)
     return flat, peak, norm
 
 
@@ -299,7 +307,7 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     before clipping.  The unclipped gradients are never stored."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     dev = _on_gpu(words)
-    g = _table(grads, written=True)
+    g = _table(grads)
     if dev != g.device:
         _refuse(f"qsgd_decode_clip: words on {dev}, gradients on {g.device}")
     if words.dtype != torch.int32 or not words.is_contiguous():
@@ -314,4 +322,5 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     ws = g._workspace()
     _call("gc_qsgd_decode_clip", dev, words.data_ptr(), g.n, nt.data_ptr(), int(bits), C.byref(lanes), float(alpha),
           g._use(), code, max_norm, out.data_ptr(), _at(ws))
+    g._written()
     return out

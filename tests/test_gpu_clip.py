@@ -708,3 +708,54 @@ def test_short_lists_touch_no_workspace(p):
     assert lib.gc_grad_flatten_clip(g._ref, flat.data_ptr(), code, 0.5, peak.data_ptr(), norm.data_ptr(),
                                     ws.data_ptr(), st) == 0
     assert bool((ws == 7).all())
+
+
+def test_every_write_is_told_to_autograd():
+    """Lists, tables of tensors and the bucket: a tensor saved for a backward is not changed unnoticed."""
+    sizes = [5000, 0, 33]
+    src = views(carve(sizes, [F32, BF16, F16], seed=181))
+    words, _, scale = packed(sum(sizes), 4, 1, seed=3)
+    read = [t._version for t in src]
+    for make in (list, gcodec.Grads):
+        for write in (lambda o: gcodec.clip_grads(src, make(o), 1.0), lambda o: gcodec.clip_grads(make(src), make(o), 1.0),
+                      lambda o: gcodec.qsgd_decode_clip(words, scale, 4, make(o), 1.0),
+                      lambda o: (lambda g: gcodec.clip_grads(g, g, 0.5))(make(o))):
+            outs = [torch.ones(s, device=DEV) for s in sizes]
+            w = torch.full((sizes[0],), 2.0, device=DEV, requires_grad=True)
+            y = (w * outs[0]).sum()  # keeps outs[0]
+            before = [o._version for o in outs]
+            write(outs)
+            assert all(o._version > v for o, v in zip(outs, before))
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    flat = torch.zeros(sum(sizes), device=DEV)
+    view, before = flat[3:9], flat._version
+    gcodec.flatten_clip(gcodec.Grads(src), 1.0, flat=flat)
+    assert flat._version > before and view._version == flat._version
+    assert [t._version for t in src] == read  # reading is none
+
+
+def test_a_call_that_writes_nothing_tells_autograd_nothing():
+    """Refused, or raised by error_if_nonfinite ahead of the write."""
+    src = views(carve([5000, 33], [F32, BF16], seed=182))
+    outs, y = [torch.ones(5000, device=DEV), torch.ones(33, device=DEV)], torch.ones(5033, device=DEV)
+    words, _, scale = packed(5033, 4, 1, seed=3)
+    before = [o._version for o in outs + [y]]
+    E = gcodec.GCodecError
+    for make in (list, gcodec.Grads):
+        with pytest.raises(E, match="sizes"):
+            gcodec.clip_grads([y[:5001], y[5001:]], make(outs), 1.0)
+        with pytest.raises(E, match="tensors into"):
+            gcodec.clip_grads([y], make(outs), 1.0)
+        with pytest.raises(E, match="needed"):
+            gcodec.qsgd_decode_clip(words[:8], scale, 4, make(outs), 1.0)
+        with pytest.raises(E, match="lanes"):
+            gcodec.qsgd_decode_clip(words, scale, 4, make(outs), 1.0, lanes=codec.qsgd_layout(5033, 2))
+    with pytest.raises(E, match="flat bucket"):
+        gcodec.flatten_clip([y], 1.0, flat=y)
+    src[0][9] = math.nan
+    for make in (list, gcodec.Grads):
+        with pytest.raises(RuntimeError, match="not finite"):
+            gcodec.clip_grads(src, make(outs), 1.0, error_if_nonfinite=True)
+    assert [o._version for o in outs + [y]] == before
+    assert all(bool((o == 1).all()) for o in outs)
