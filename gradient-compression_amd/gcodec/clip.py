@@ -106,7 +106,7 @@ class Grads:
             _refuse("Grads: made under graph capture; make the table before it")
         rec = torch.frombuffer(bytearray(self._host), dtype=torch.int64)
         self._rec = rec.to(self.device)  # complete when this returns, whatever stream reads it
-        self._home = _raw_stream(self.device.index)
+        self._streams = set()  # those that the allocator was told of
         self.struct.rec = self._rec.data_ptr()
         self._tensors = [t.detach() for t in tensors]  # their memory and their version counters
 
@@ -119,7 +119,7 @@ class Grads:
             return None
         self._tensors = tensors
         self._rec = torch.empty(len(self._host) // 8, dtype=torch.int64, device=self.device)
-        self._home = None
+        self._streams = None
         self.struct.rec = rec = self._rec.data_ptr()
         _call("gc_grads_fill", self.device, self._ref, rec)
         return self
@@ -151,10 +151,15 @@ class Grads:
         return True
 
     def _use(self):
-        """The table for a launch; the allocator is told of a stream other than the one the table was made on."""
-        if self._home is not None and _raw_stream(self.device.index) != self._home:
+        """The table for a launch.  A kept table may be the last to hold its tensors and be dropped while a kernel
+        runs on a stream other than theirs: the allocator is told, once for each stream, and gives their memory
+        out again only behind that stream's work."""
+        if self._streams is not None and (raw := _raw_stream(self.device.index)) not in self._streams:
             if not torch.cuda.is_current_stream_capturing():
-                self._rec.record_stream(torch.cuda.current_stream(self.device))
+                stream = torch.cuda.current_stream(self.device)
+                for t in (self._rec, *self._tensors):
+                    t.record_stream(stream)
+                self._streams.add(raw)
         return self._ref
 
     def _written(self):

@@ -759,3 +759,26 @@ def test_a_call_that_writes_nothing_tells_autograd_nothing():
             gcodec.clip_grads(src, make(outs), 1.0, error_if_nonfinite=True)
     assert [o._version for o in outs + [y]] == before
     assert all(bool((o == 1).all()) for o in outs)
+
+
+def test_dropped_table_holds_its_memory_for_the_stream():
+    """A table that was the last to hold its tensors, used on a side stream and dropped while that stream still
+    waits: the tensors' memory is not given out again before the stream has run."""
+    side, n = torch.cuda.Stream(), 1 << 20
+    for write in (False, True):
+        src, out = [torch.full((n,), 2.0, device=DEV)], [torch.zeros(n, device=DEV)]
+        gi, go = gcodec.Grads(src), gcodec.Grads(out)
+        held = {t.data_ptr() for t in (src + out if write else src)}
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)  # 0.01 s at least
+            norm = gcodec.clip_grads(gi, go, INF) if write else gcodec.grad_norm(gi, INF)
+        del src, gi
+        if write:
+            del out, go
+        assert not side.query()
+        later = [torch.full((n,), 9.0, device=DEV) for _ in range(4)]  # on the current stream, ahead of the side's work
+        assert not held & {t.data_ptr() for t in later}
+        torch.cuda.synchronize()
+        # clip_grads takes the 2-norm: 2^20 twos have 2 * 2^10
+        assert float(norm) == (2048.0 if write else 2.0) and all(bool((t == 9).all()) for t in later)
