@@ -28,16 +28,17 @@ const at::Tensor *item(PyObject *o, bool of_grads)
     return of_grads ? &t.grad() : &t;
 }
 
-// gather(tensors, of_grads, ordered, plan, grads): fills the gc_grads at the
-// address `grads` by the gc_grads_plan at the address `plan`
+// gather(tensors, of_grads, ordered, written, plan, grads): fills the gc_grads at
+// the address `grads` by the gc_grads_plan at the address `plan`
 // -> (device index, host records, order); None without any gradient.
 // ordered: a tensor's elements are taken row by row (else in any dense order)
+// written: they may be written or kept, so a copy-on-write tensor gets its own memory
 PyObject *gather(PyObject *, PyObject *args)
 {
     PyObject *list;
-    int of_grads, ordered;
+    int of_grads, ordered, written;
     unsigned long long plan, out;
-    if (!PyArg_ParseTuple(args, "OppKK", &list, &of_grads, &ordered, &plan, &out))
+    if (!PyArg_ParseTuple(args, "OpppKK", &list, &of_grads, &ordered, &written, &plan, &out))
         return nullptr;
     PyObject *seq = PySequence_Fast(list, "not a list of dense tensors");
     if (!seq)
@@ -89,7 +90,7 @@ PyObject *gather(PyObject *, PyObject *args)
                 goto done;
             }
             sizes.push_back((uint64_t)t->numel());
-            ptrs.push_back(t->const_data_ptr());
+            ptrs.push_back(written ? t->mutable_data_ptr() : t->const_data_ptr());
             types.push_back(type == at::kFloat ? GC_F32 : type == at::kHalf ? GC_F16 : GC_BF16);
         }
         if (types.empty()) {

@@ -100,7 +100,7 @@ class Grads:
 
     def __init__(self, tensors):
         tensors = list(tensors)
-        if not self._build(tensors):
+        if not self._build(tensors, written=True):
             _refuse("Grads: empty tensor list")
         if torch.cuda.is_current_stream_capturing():
             _refuse("Grads: made under graph capture; make the table before it")
@@ -111,11 +111,11 @@ class Grads:
         self._tensors = [t.detach() for t in tensors]  # their memory and their version counters
 
     @classmethod
-    def _of_call(cls, tensors, of_grads=False, ordered=True):
+    def _of_call(cls, tensors, of_grads=False, ordered=True, written=False):
         """The table of a list (of_grads: of the list's gradients; None if there are none) for the length of
         one call, filled on the current stream."""
         self = cls.__new__(cls)
-        if not self._build(tensors, of_grads, ordered):
+        if not self._build(tensors, of_grads, ordered, written):
             return None
         self._tensors = tensors
         self._rec = torch.empty(len(self._host) // 8, dtype=torch.int64, device=self.device)
@@ -124,15 +124,16 @@ class Grads:
         _call("gc_grads_fill", self.device, self._ref, rec)
         return self
 
-    def _build(self, tensors, of_grads=False, ordered=True) -> bool:
-        """ordered: element i of a tensor is its i-th in row-major order (else any dense order does)"""
+    def _build(self, tensors, of_grads=False, ordered=True, written=False) -> bool:
+        """ordered: element i of a tensor is its i-th in row-major order (else any dense order does)
+        written: the tensors may be written, or are kept (a copy-on-write one gets its own memory)"""
         lib = _lib.load()
         self.struct = _lib.gc_grads()
         self._ref = C.byref(self.struct)
         self._of_grads = of_grads
         try:
-            got = _lib.tensor_list().gather(tensors, of_grads, ordered, C.cast(lib.gc_grads_plan, C.c_void_p).value,
-                                            C.addressof(self.struct))
+            got = _lib.tensor_list().gather(tensors, of_grads, ordered, written,
+                                            C.cast(lib.gc_grads_plan, C.c_void_p).value, C.addressof(self.struct))
         except LookupError as e:
             raise _lib.GCodecError(_lib.GC_ENODEV, f"gcodec runs on the GPU only: {e}; there is no CPU fallback") from None
         except ValueError as e:
@@ -175,15 +176,15 @@ class Grads:
         return torch.empty((), dtype=dtype, device=self.device)
 
 
-def _table(grads, ordered=True) -> Grads:
-    """The table of a list."""
+def _table(grads, ordered=True, written=False) -> Grads:
+    """The table of a list (written: whose tensors this call writes)."""
     if isinstance(grads, Grads):
         return grads
     if isinstance(grads, torch.Tensor):
         grads = [grads]
     elif not isinstance(grads, (list, tuple)):
         grads = list(grads)
-    g = Grads._of_call(grads, False, ordered)
+    g = Grads._of_call(grads, False, ordered, written)
     if g is None:
         _refuse("Grads: empty tensor list")
     return g
@@ -258,8 +259,8 @@ def clip_grads(grads, out, max_norm: float, norm_type: float = 2.0, error_if_non
     tensor may be clipped onto itself; apart from that the tensors of `out`
     share no memory with each other or with `grads`."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
-    src = _table(grads)
-    dst = src if out is grads else _table(out)
+    dst = _table(out, written=True)  # ahead of src: a tensor in both has its own memory by then
+    src = dst if out is grads else _table(grads)
     return _clip(src, dst, max_norm, code, error_if_nonfinite, group, "clip_grads")
 
 
@@ -269,7 +270,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     torch.nn.utils.clip_grad_norm_, with the norm held in 64 bits."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    src = Grads._of_call(parameters, True, False)
+    src = Grads._of_call(parameters, True, False, True)
     if src is None:
         dev = parameters[0].device if parameters else None
         norm = torch.zeros((), dtype=torch.float64, device=dev)
@@ -312,7 +313,7 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
     before clipping.  The unclipped gradients are never stored."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     dev = _on_gpu(words)
-    g = _table(grads)
+    g = _table(grads, written=True)
     if dev != g.device:
         _refuse(f"qsgd_decode_clip: words on {dev}, gradients on {g.device}")
     if words.dtype != torch.int32 or not words.is_contiguous():

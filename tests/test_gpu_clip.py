@@ -782,3 +782,32 @@ def test_dropped_table_holds_its_memory_for_the_stream():
         torch.cuda.synchronize()
         # clip_grads takes the 2-norm: 2^20 twos have 2 * 2^10
         assert float(norm) == (2048.0 if write else 2.0) and all(bool((t == 9).all()) for t in later)
+
+
+def test_copy_on_write_tensors_are_written_alone():
+    """A lazy clone shares its source's memory until one of the two is written."""
+    n = 5000
+    words, _, scale = packed(n, 4, 1, seed=3)
+    for make in (list, gcodec.Grads):
+        for write in (lambda o: gcodec.clip_grads([torch.full((n,), 3.0, device=DEV)], make(o), 1.0),
+                      lambda o: gcodec.qsgd_decode_clip(words, scale, 4, make(o), 1.0),
+                      lambda o: (lambda g: gcodec.clip_grads(g, g, 0.5))(make(o))):
+            a = torch.full((n,), 2.0, device=DEV)
+            b = torch._lazy_clone(a)
+            write([b])
+            assert bool((a == 2).all()) and not bool((b == 2).any())
+    w, a = torch.nn.Parameter(torch.zeros(n, device=DEV)), torch.full((n,), 2.0, device=DEV)
+    w.grad = torch._lazy_clone(a)
+    gcodec.clip_grad_norm_([w], 1.0)
+    assert bool((a == 2).all()) and not bool((w.grad == 2).any())
+    flat = torch._lazy_clone(a)
+    gcodec.flatten_clip([torch.full((n,), 3.0, device=DEV)], 1.0, flat=flat)
+    assert bool((a == 2).all()) and not bool((flat == 2).any())
+    # partly in place: the clone is both an input and its own output
+    b, c = torch._lazy_clone(a), torch.empty(7, device=DEV)
+    gcodec.clip_grads([b, torch.ones(7, device=DEV)], [b, c], 1.0)
+    assert bool((a == 2).all())
+    norm = math.sqrt(4.0 * n + 7)
+    close_values([b, c], [np.full(n, 2.0 * coef64(norm, 1.0)), np.full(7, coef64(norm, 1.0))])
+    b = torch._lazy_clone(a)  # a read one is left as it is
+    assert float(gcodec.grad_norm([b], INF)) == 2.0 and torch._C._is_cow_tensor(b)
