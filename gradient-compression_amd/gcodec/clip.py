@@ -54,9 +54,9 @@ def _norm_code(norm_type) -> int:
     return 1
 
 
-def _limit(max_norm) -> float:
+def _limit(max_norm, name: str = "max_norm") -> float:
     if not isinstance(max_norm, numbers.Real) or not float(max_norm) >= 0.0:
-        _refuse(f"max_norm must be a number at or above 0, got {max_norm!r}")
+        _refuse(f"{name} must be a number at or above 0, got {max_norm!r}")
     return float(max_norm)
 
 

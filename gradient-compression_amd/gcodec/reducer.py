@@ -80,8 +80,10 @@ class Reducer:
         if topology is not None and group is not None:
             raise ValueError("topology spans the default process group; pass one or the other")
         self._fused = fused
-        self._max_grad_norm = max_grad_norm
-        self._local_max_norm = local_max_norm
+        # refused here, not in a step that other ranks have entered
+        limit = _hip_clip._limit
+        self._max_grad_norm = None if max_grad_norm is None else limit(max_grad_norm, "max_grad_norm")
+        self._local_max_norm = None if local_max_norm is None else limit(local_max_norm, "local_max_norm")
         self.grad_norm = None        # norm of the last averaged gradient before max_grad_norm
         self.local_grad_norm = None  # norm of this rank's last gradient before local_max_norm
         # a codec other than the HIP one brings its own clip operators, or has none

@@ -115,3 +115,18 @@ def test_a_codec_without_clip_operators_is_refused():
     for kw in (dict(max_grad_norm=1.0), dict(local_max_norm=1.0)):
         with pytest.raises(ValueError, match="clip operators"):
             R.QSGDMaxNormReducer(torch.device("cpu"), None, quantization_level=4, codec=oracle_codec, **kw)
+
+
+@pytest.mark.parametrize("option", ["max_grad_norm", "local_max_norm"])
+@pytest.mark.parametrize("bad", [-1.0, float("nan"), float("-inf"), "1", [1.0]])
+def test_a_limit_is_checked_when_the_reducer_is_made(option, bad):
+    """Not in the step, behind its collectives and its writes to grad_out."""
+    from _gloo_workers import make_reducer
+
+    from gcodec import GCodecError
+
+    for name in ("qsgd", "ts", "ms", "randk", "randk_ts"):
+        with pytest.raises(GCodecError, match=option):
+            make_reducer(name, codec=_codec(), **{option: bad})
+    for good in (0, 0.5, float("inf"), np.float32(2.0), None):
+        make_reducer("qsgd", codec=_codec(), **{option: good})
