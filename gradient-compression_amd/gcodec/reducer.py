@@ -42,6 +42,8 @@ from . import codec as _hip_codec
 from . import compressors as C
 from .rng import default_generator
 
+_CLIP_TYPES = frozenset((torch.float32, torch.float16, torch.bfloat16))
+
 
 class _NullTimer:
     def __call__(self, label, epoch=-1.0, verbosity=1):
@@ -164,7 +166,10 @@ class Reducer:
         if self._local_max_norm is not None:
             grad_in = list(grad_in)
             with self._timer("reduce.flat_pack"):
-                buf, norm, self.local_grad_norm = self._clip.flatten_clip(grad_in, self._local_max_norm)
+                rows = grad_in  # row by row, as TensorBuffer takes them
+                if not all(map(torch.Tensor.is_contiguous, rows)):
+                    rows = [t.contiguous() for t in rows]
+                buf, norm, self.local_grad_norm = self._clip.flatten_clip(rows, self._local_max_norm)
             return TensorBuffer.of_flat(grad_in, buf), norm
         segs = self._segments(grad_in)
         if segs is None:
@@ -175,12 +180,31 @@ class Reducer:
             buf, norm = self._codec.segments_flatten_absmax(segs)
         return TensorBuffer.of_flat(grad_in, buf), norm
 
-    def _clip_out(self, grad_out):
+    @staticmethod
+    def _clip_list(grad_out, device):
+        """grad_out for the clip operators, which write contiguous tensors of three types on one device
+        -> (list, the (stand-in, tensor) pairs of those that are not)"""
+        outs = list(grad_out)
+        if (all(map(torch.Tensor.is_contiguous, outs)) and _CLIP_TYPES.issuperset(t.dtype for t in outs)
+                and frozenset(map(torch.Tensor.get_device, outs)) == {device.index if device.index is not None else -1}):
+            return outs, ()
+        held = []
+        for i, t in enumerate(outs):
+            if not (t.is_contiguous() and t.dtype in _CLIP_TYPES and t.device == device):
+                outs[i] = torch.empty(t.shape, dtype=t.dtype if t.dtype in _CLIP_TYPES else torch.float32, device=device)
+                held.append((outs[i], t))
+        return outs, held
+
+    def _clip_out(self, grad_out, device):
         """max_grad_norm on a written grad_out."""
         if self._max_grad_norm is not None:
             with self._timer("reduce.clip", verbosity=2):
-                outs = list(grad_out)
+                outs, held = self._clip_list(grad_out, device)
+                for x, t in held:
+                    x.copy_(t)
                 self.grad_norm = self._clip.clip_grads(outs, outs, self._max_grad_norm)
+                for x, t in held:
+                    t.copy_(x)
 
     def _max_norm(self, flat, local=None, idx=None):
         with self._timer("reduce.norm", verbosity=2):
@@ -247,8 +271,11 @@ class QSGDMaxNormReducer(Reducer):
         bits = self.n_bits(norm) + self.n_bits(words)
         if self._max_grad_norm is not None:  # the norm is taken from the words: decode + 1/W + clipping in one write
             with self._timer("reduce.decompress", verbosity=2):
-                self.grad_norm = self._clip.qsgd_decode_clip(words, norm, self._quantization_level, list(grad_out),
+                outs, held = self._clip_list(grad_out, words.device)
+                self.grad_norm = self._clip.qsgd_decode_clip(words, norm, self._quantization_level, outs,
                                                              self._max_grad_norm, world=W, alpha=1.0 / W)
+                for x, t in held:
+                    t.copy_(x)
             return bits
         out_segs = self._segments(grad_out)
         with self._timer("reduce.decompress", verbosity=2):
@@ -356,7 +383,7 @@ class GlobalRandKMaxNormReducer(Reducer):
         pair = self._segment_pair(grad_in, grad_out)
         if pair is not None:
             bits = self._reduce_segments(comp, *pair)
-            self._clip_out(grad_out)
+            self._clip_out(grad_out, pair[1].device)
             return bits
         flat, _ = self._flat_pack(grad_in)
         n = flat.buffer.numel()
@@ -385,7 +412,7 @@ class GlobalRandKMaxNormReducer(Reducer):
             comp.decode(norm, words, k, world=W, alpha=1.0, idx=idx, out=flat.buffer)
         with self._timer("reduce.setgrad", verbosity=2):
             self._setgrad_scaled(flat, grad_out, 1.0 / W)
-        self._clip_out(grad_out)
+        self._clip_out(grad_out, words.device)
         return bits
 
 
@@ -444,7 +471,7 @@ class QSGDMaxNormTwoScaleReducer(Reducer):
         with self._timer("reduce.setgrad", verbosity=2):
             if out_segs is None:
                 self._setgrad(flat, grad_out)
-        self._clip_out(grad_out)
+        self._clip_out(grad_out, words.device)
         return bits
 
 
@@ -497,7 +524,7 @@ class GlobalRandKMaxNormTwoScaleReducer(QSGDMaxNormTwoScaleReducer):
         pair = self._segment_pair(grad_in, grad_out)
         if pair is not None and hasattr(comp, "decode_scatter_segments"):
             bits = self._reduce_segments(comp, *pair)
-            self._clip_out(grad_out)
+            self._clip_out(grad_out, pair[1].device)
             return bits
         flat, _ = self._flat_pack(grad_in)
         n = flat.buffer.numel()
@@ -508,7 +535,7 @@ class GlobalRandKMaxNormTwoScaleReducer(QSGDMaxNormTwoScaleReducer):
             comp.decode(norm, words, mask, k, world=W, alpha=1.0, idx=idx, out=flat.buffer)
         with self._timer("reduce.setgrad", verbosity=2):
             self._setgrad_scaled(flat, grad_out, 1.0 / W)
-        self._clip_out(grad_out)
+        self._clip_out(grad_out, words.device)
         return bits
 
 

@@ -811,3 +811,51 @@ def test_copy_on_write_tensors_are_written_alone():
     close_values([b, c], [np.full(n, 2.0 * coef64(norm, 1.0)), np.full(7, coef64(norm, 1.0))])
     b = torch._lazy_clone(a)  # a read one is left as it is
     assert float(gcodec.grad_norm([b], INF)) == 2.0 and torch._C._is_cow_tensor(b)
+
+
+@pytest.mark.parametrize("name,kw", REDUCERS)
+def test_reducer_options_take_any_strides(name, kw):
+    """channels_last, transposed and sliced gradients, as without the options; outputs also of wider types
+    and on the host."""
+    shapes_ = [(8, 6, 5, 4), (64,), (30, 40), (0, 3), (7, 9)]
+    rng = np.random.default_rng(191)
+    plain = [torch.from_numpy(rng.standard_normal(s).astype(np.float32) * 0.01).to(DEV) for s in shapes_]
+
+    def odd(ts):
+        return [ts[0].contiguous(memory_format=torch.channels_last), ts[1], ts[2].t().contiguous().t(), ts[3],
+                torch.cat([ts[4], ts[4]], 1)[:, :9]]
+
+    def outs():
+        ones = odd([torch.full(s, 9.0, device=DEV) for s in shapes_])
+        ones[1] = ones[1].double()
+        if not name.startswith("GlobalRandK"):  # whose setgrad adds in place, on the GPU only
+            ones[4] = ones[4].cpu()
+        return ones
+
+    ins = odd(plain)
+    assert [t.is_contiguous() for t in ins] == [False, True, False, True, False]
+    want = outs()
+    bits = reducer(name, kw).reduce(ins, want)
+    same = [torch.full_like(t, 9.0) for t in plain]
+    reducer(name, kw).reduce(plain, same)
+    for a, b in zip(want, same):
+        assert torch.equal(a.to(DEV, F32), b)
+    n = norm64(f64(same), 2)
+    got = outs()
+    r = reducer(name, kw, local_max_norm=INF, max_grad_norm=2 * n)  # under both limits: the same bits
+    assert r.reduce(ins, got) == bits
+    close_norm(r.local_grad_norm, norm64(f64(plain), 2))
+    close_norm(r.grad_norm, n, roundings=5)
+    for a, b in zip(got, want):
+        assert a.stride() == b.stride() and torch.equal(a, b)
+    got = outs()
+    r = reducer(name, kw, max_grad_norm=0.5 * n)
+    r.reduce(ins, got)
+    # a clipped value is a float32's before it is any wider type's
+    close_values([t.to(DEV, F32) for t in got], [x * coef64(n, 0.5 * n) for x in f64(same)], extra=8)
+    before = [torch.empty_like(t) for t in plain]
+    gcodec.clip_grads(plain, before, 0.05)
+    reducer(name, kw).reduce(before, same)
+    reducer(name, kw, local_max_norm=0.05).reduce(ins, got)
+    for a, b in zip(got, same):
+        assert torch.equal(a.to(DEV, F32), b)
