@@ -264,11 +264,15 @@ def clip_grads(grads, out, max_norm: float, norm_type: float = 2.0, error_if_non
     return _clip(src, dst, max_norm, code, error_if_nonfinite, group, "clip_grads")
 
 
-def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, group=None):
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                    foreach=None, *, group=None):
     """Clips the gradients of `parameters` in place; -> their norm before it (a
     float32 scalar tensor, 0 without any gradient).  As
-    torch.nn.utils.clip_grad_norm_, with the norm held in 64 bits."""
+    torch.nn.utils.clip_grad_norm_, with the norm held in 64 bits; `foreach`,
+    which picks one of torch's two implementations, changes nothing here."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
+    if foreach not in (None, True, False):
+        _refuse(f"foreach must be None, True or False, got {foreach!r} (group= is given by name)")
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     src = Grads._of_call(parameters, True, False, True)
     if src is None:

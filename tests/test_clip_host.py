@@ -233,3 +233,19 @@ def test_ranks_join_their_totals():
     args = [port, root, os.path.join(root, "gradient-compression_amd")]
     ps = [subprocess.Popen([sys.executable, "-c", WORKER, str(r)] + args) for r in range(2)]
     assert [p.wait(timeout=120) for p in ps] == [0, 0]
+
+
+def test_the_trainer_call_keeps_its_arguments():
+    """torch.nn.utils.clip_grad_norm_'s own, in its order; foreach chooses between torch's two ways, here one."""
+    import inspect
+
+    theirs = list(inspect.signature(torch.nn.utils.clip_grad_norm_).parameters)
+    mine = inspect.signature(clip.clip_grad_norm_).parameters
+    assert list(mine)[:len(theirs)] == theirs
+    assert mine["group"].kind is inspect.Parameter.KEYWORD_ONLY
+    w = torch.nn.Parameter(torch.ones(4))
+    for foreach in (None, True, False):
+        assert clip.clip_grad_norm_([w], 1.0, 2.0, False, foreach).item() == 0.0
+        assert clip.clip_grad_norm_([w], 1.0, foreach=foreach).item() == 0.0
+    with pytest.raises(_lib.GCodecError, match="foreach"):
+        clip.clip_grad_norm_([w], 1.0, 2.0, False, object())  # a group is given by name
