@@ -859,3 +859,24 @@ def test_reducer_options_take_any_strides(name, kw):
     reducer(name, kw, local_max_norm=0.05).reduce(ins, got)
     for a, b in zip(got, same):
         assert torch.equal(a.to(DEV, F32), b)
+
+
+@pytest.mark.parametrize("shape,perm", [((3, 4, 5), (0, 1, 2)), ((3, 4, 5), (2, 0, 1)), ((2, 3, 4, 5), (0, 2, 3, 1)),
+                                        ((1, 4, 1), (2, 1, 0)), ((4, 1, 6), (1, 2, 0)), ((0, 3), (1, 0)), ((6000, 7), (1, 0))])
+def test_dense_orders_of_gradients(shape, perm):
+    """Any order of the dimensions, with sizes of one and none: the norm and the clip in place take them all."""
+    rng = np.random.default_rng(201)
+    for t in (F32, BF16, F16):
+        w = torch.nn.Parameter(torch.zeros(shape, dtype=t, device=DEV).permute(perm))
+        g = torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(DEV, t).permute(perm)
+        w.grad = g
+        x = g.cpu().double().numpy().copy()
+        n = norm64([x.reshape(-1)], 2)
+        close_norm(gcodec.grad_norm([g]), n)
+        close_norm(gcodec.clip_grad_norm_([w], 0.3), n)
+        assert w.grad.stride() == g.stride() and w.grad.data_ptr() == g.data_ptr()
+        close_values([w.grad.contiguous()], [x.reshape(-1) * coef64(n, 0.3)])
+    # one tensor's rows, columns or repetitions are not dense
+    for bad in (torch.zeros(4, 6, device=DEV)[:, :3], torch.zeros(4, 1, device=DEV).expand(4, 5), torch.zeros(9, device=DEV)[::2]):
+        with pytest.raises(gcodec.GCodecError, match="not dense"):
+            gcodec.grad_norm([bad])
