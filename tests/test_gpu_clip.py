@@ -880,3 +880,108 @@ def test_dense_orders_of_gradients(shape, perm):
     for bad in (torch.zeros(4, 6, device=DEV)[:, :3], torch.zeros(4, 1, device=DEV).expand(4, 5), torch.zeros(9, device=DEV)[::2]):
         with pytest.raises(gcodec.GCodecError, match="not dense"):
             gcodec.grad_norm([bad])
+
+
+# ---------------------------------------------------------------------------
+# lists as large as a model's, checked on the device
+# ---------------------------------------------------------------------------
+LARGE = {  # odd sizes and ends; more work than one round of the launch, more bytes than the cache in front of the memory
+    "few": [100_000_003, 0, 17, 60_000_000, 5001],
+    "few and 1200 small": [30_000_001, *(1 + i % 9 for i in range(600)), 90_000_007, *(i % 700 for i in range(600)), 40_000_005],
+    "large, then a run of ones": [25_000_001] + [1 + i % 3 for i in range(2500)],
+}
+
+
+def guarded(sizes, dtype):
+    """Tensors at odd offsets of one buffer with 7.0 between them; the buffer and a mask of what lies between."""
+    buf = torch.full((sum(sizes) + 3 * len(sizes) + 8,), 7.0, dtype=dtype, device=DEV)
+    between = torch.ones(buf.numel(), dtype=torch.bool, device=DEV)
+    at, out = 1, []
+    for s in sizes:
+        out.append(buf[at:at + s])
+        between[at:at + s] = False
+        at += s + 3
+    return out, buf, between
+
+
+def close_on_device(got, want, extra=0):
+    """close_values for tensors end to end, a part at a time"""
+    u, rel = UNIT[got.dtype], (2 + extra) * 2.0 ** -24 * (1 + 2.0 ** -6)
+    rel += u * (1 + 2.0 ** -6) if got.dtype != F32 else 0.0
+    for g, w in zip(got.split(1 << 26), want.split(1 << 26)):
+        err = (g.double() - w).abs_()
+        tol = w.abs().mul_(rel).add_(TINY[got.dtype] * 0.5 + (1 + extra) * 2.0 ** -150)
+        assert bool((err <= tol).all())
+
+
+def norm_on_device(x, p):
+    """in 64 bits; its sums are within 2^-40 of the exact ones (a tree of n < 2^28 terms)"""
+    if p == INF:
+        return float(x.abs().max())
+    return math.sqrt(float(x.square().sum())) if p == 2 else float(x.abs().sum())
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("name", list(LARGE))
+def test_large_lists(name, kind, p):
+    """Norms, list to list, in place and into the bucket."""
+    sizes = LARGE[name]
+    src, _, _ = guarded(sizes, kind)
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    for i, t in enumerate(src):
+        if t.numel():
+            t.copy_(torch.randn(t.numel(), generator=gen, device=DEV) * 2.0 ** (i % 5 - 2))
+    x = torch.cat(src).double()
+    n = norm_on_device(x, p)
+    c = coef64(n, 0.3 * n)
+    total, each = gcodec.grad_norm(src, p, per_tensor=True)
+    close_norm(total, n)
+    mine = each.tolist()
+    at = 0
+    for k, s in enumerate(sizes):
+        if s > 1000 or k % 97 == 0:
+            close_norm(mine[k], norm_on_device(x[at:at + s], p) if s else 0.0)
+        at += s
+    outs, buf, between = guarded(sizes, BF16)
+    close_norm(gcodec.clip_grads(src, outs, 0.3 * n, p), n)
+    x.mul_(c)
+    close_on_device(torch.cat(outs), x)
+    assert bool((buf[between] == 7).all())
+    del outs, buf, between
+    flat, peak, total = gcodec.flatten_clip(src, 0.3 * n, p)
+    close_norm(total, n)
+    close_on_device(flat, x)
+    assert float(peak) == float(flat.abs().max())
+    del flat
+    table = gcodec.Grads(src)
+    close_norm(gcodec.clip_grads(table, table, 0.3 * n, p), n)
+    close_on_device(torch.cat(src), x)
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("name,kind,bits,world", [("few", BF16, 8, 8), ("few and 1200 small", BF16, 8, 8),
+                                                  ("few and 1200 small", F32, 4, 1), ("few", F32, 16, 1),
+                                                  ("large, then a run of ones", F32, 4, 3)])
+def test_decode_of_large_lists(name, kind, bits, world, p):
+    sizes = LARGE[name]
+    n, s = sum(sizes), (1 << bits) - 1
+    # every place has its own level: a product with an odd number, folded into -world s .. world s
+    i = torch.arange(n, dtype=torch.int64, device=DEV)
+    q = ((i * 2_654_435_761 + 12_345) >> 7) % (2 * world * s + 1) - world * s
+    del i
+    lanes = codec.qsgd_layout(n, bits, world)
+    words = torch.zeros(lanes.plane_words, dtype=torch.int64, device=DEV)
+    for k in range(lanes.per_word):
+        part = q[k * lanes.plane_words:(k + 1) * lanes.plane_words]
+        words[:part.numel()] += (part + world * s) << (k * lanes.bits)
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+    norm = torch.tensor([0.02], dtype=F32, device=DEV)
+    x = q.double().mul_(float(norm) / s / world)
+    del q
+    want = norm_on_device(x, p)
+    outs, buf, between = guarded(sizes, kind)
+    total = gcodec.qsgd_decode_clip(words, norm, bits, outs, 0.37 * want, p, world=world, alpha=1.0 / world)
+    close_norm(total, want, roundings=5)
+    close_on_device(torch.cat(outs), x.mul_(coef64(want, 0.37 * want)), extra=8)
+    assert bool((buf[between] == 7).all())
