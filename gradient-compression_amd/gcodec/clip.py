@@ -127,13 +127,13 @@ class Grads:
     def _build(self, tensors, of_grads=False, ordered=True, written=False) -> bool:
         """ordered: element i of a tensor is its i-th in row-major order (else any dense order does)
         written: the tensors may be written, or are kept (a copy-on-write one gets its own memory)"""
-        lib = _lib.load()
+        lib, self._lists = _lib.load(), _lib.tensor_list()
         self.struct = _lib.gc_grads()
         self._ref = C.byref(self.struct)
         self._of_grads = of_grads
         try:
-            got = _lib.tensor_list().gather(tensors, of_grads, ordered, written,
-                                            C.cast(lib.gc_grads_plan, C.c_void_p).value, C.addressof(self.struct))
+            got = self._lists.gather(tensors, of_grads, ordered, written,
+                                     C.cast(lib.gc_grads_plan, C.c_void_p).value, C.addressof(self.struct))
         except LookupError as e:
             raise _lib.GCodecError(_lib.GC_ENODEV, f"gcodec runs on the GPU only: {e}; there is no CPU fallback") from None
         except ValueError as e:
@@ -144,6 +144,7 @@ class Grads:
             return False
         index, self._host, self._order = got  # the struct points into these
         _lib.require_device(index)
+        self._index = index
         self.device = _DEVICES.get(index)
         if self.device is None:
             self.device = _DEVICES[index] = torch.device("cuda", index)
@@ -155,7 +156,7 @@ class Grads:
         """The table for a launch.  A kept table may be the last to hold its tensors and be dropped while a kernel
         runs on a stream other than theirs: the allocator is told, once for each stream, and gives their memory
         out again only behind that stream's work."""
-        if self._streams is not None and (raw := _raw_stream(self.device.index)) not in self._streams:
+        if self._streams is not None and (raw := _raw_stream(self._index)) not in self._streams:
             if not torch.cuda.is_current_stream_capturing():
                 stream = torch.cuda.current_stream(self.device)
                 for t in (self._rec, *self._tensors):
@@ -165,7 +166,7 @@ class Grads:
 
     def _written(self):
         """Tells autograd of a write to the tensors, once the launch is made."""
-        _lib.tensor_list().written(self._tensors, self._of_grads)
+        self._lists.written(self._tensors, self._of_grads)
 
     def _workspace(self, each: bool = False):
         """A call's workspace, or None where it needs none."""
