@@ -6,8 +6,8 @@
 //
 // Two passes, and nothing is kept between calls: k_grad_norm (or k_lane_norm,
 // from packed words) leaves one partial a block in the caller's workspace, and
-// every wave of the pass that writes (k_grad_scale, k_decode_clip) adds those
-// partials in one fixed order and forms c itself.  So there are no atomics, no
+// the first wave of every block of the pass that writes (k_grad_scale, k_decode_clip)
+// adds those partials in one fixed order and forms c.  So there are no atomics, no
 // tickets and no zeroed state: the result does not depend on the schedule, a
 // captured call owns all that it writes, and two calls on different streams
 // share nothing.  A list that one block can read in a few microseconds
@@ -23,8 +23,9 @@
 // them twice and writes them once; of a list beyond the 256 MB of cache in front
 // of the memory, the first read passes all but the end by the cache, and the
 // second finds that end there.  Short lists are bound by the two launches and
-// the chain partials -> c -> first load inside the second: 8.3 us for 10,000 to
-// a million elements, whatever their number.
+// the chain partials -> c -> table -> first load inside the second: 10,000 /
+// 70,000 / 250,000 / a million float32 take 8.0 / 8.5 / 8.7 / 9.9 us in 3 tensors and
+// 12.2 / 9.9 / 9.8 / 11.0 in 500.
 #include "gc_device.h"
 #include "gc_host.h"
 #include "grads.h"
@@ -55,13 +56,16 @@ constexpr unsigned kNormGrid = 512;
 // small blocks again, over more CUs (60,000 elements of 3 tensors 8.8 -> 7.9 us).
 constexpr unsigned kScaleThreads = 256;
 constexpr unsigned kScaleGrid = 16384;
-constexpr uint64_t kWaves = 8192;  // resident at once: 256 CUs of 32
+// The waves that 256 CUs hold at most, 32 each.  Blocks of 256 threads of
+// k_grad_scale come to half of it: their two tables take 33 KB of a CU's 160 KB of LDS.
+constexpr uint64_t kWaves = 8192;
 constexpr uint64_t kSpread = 1024;
 
 // Words: one block a CU adds them (128 / 256 / 512 blocks: 33.3 / 30.9 / 32.5 us
-// with the decode, whose every block reads the partials), four rounds of the
-// blocks that are resident at once decode them (2560 / 4096 / 5120 / 8192: 254 /
-// 259 / 250 / 249 us for 246M bfloat16, 96.4 / 95.3 / 95.1 / 95.2 us for 100M float32).
+// with the decode, whose every block reads the partials).  The decode's grid hardly
+// matters (2560 / 4096 / 5120 / 8192 blocks: 254 / 259 / 250 / 249 us for 246M
+// bfloat16, 96.4 / 95.3 / 95.1 / 95.2 us for 100M float32): whole rounds, four, of
+// the 1280 blocks that are resident at once (90 registers: five a CU).
 constexpr unsigned kLaneGrid = 256;
 constexpr unsigned kDecodeGrid = 5120;
 
@@ -1147,7 +1151,10 @@ static uint64_t held_bytes(const gc_grads *g)
 
 // The elements of a wave's tile: `most`, or as few as spread a short list over
 // the chip (over the waves of the one block that does all of it); the least for
-// tensors that are small on the whole, which a lane at a time takes.  Halved
+// tensors that are small on the whole, which a lane at a time takes.  That goes by
+// the list's average: a run of tiny tensors in a list that is large on the whole is
+// walked a tensor at a time (clipping 50M elements and 2000 tensors of one takes
+// 2.0 ms, 90 us as one tensor; their norm 0.76 ms and 32 us).  Halved
 // while the list has less than 16384 of the smaller tiles, but to 256 only below
 // 4096 (2M float32: clip 12.7 us at 512, 15.1 at 256; 7M 20.8 at 512, 21.9 at 1024;
 // 12M: norm 12.5 at 1024, 15.2 at 2048) and, for 16-bit norms, to 2048 and 1024

@@ -219,7 +219,8 @@ def _norm_into(g: Grads, code: int, norm, each=None, total=None):
 def grad_norm(grads, norm_type: float = 2.0, per_tensor: bool = False, error_if_nonfinite: bool = False, group=None):
     """The norm of all gradients together, a float32 scalar tensor; with
     per_tensor=True (norm, norms), `norms` a float32 tensor of each tensor's own
-    (with a group: of this rank's part).  No gradients at all have norm 0."""
+    (with a group: of this rank's part).  Empty tensors have norm 0; a list of no
+    tensors, which names no device, is refused."""
     code = _norm_code(norm_type)
     g = _table(grads, ordered=False)
     norm = g._scalar()
@@ -315,7 +316,9 @@ def qsgd_decode_clip(words, norm, bits: int, grads, max_norm: float, norm_type: 
                      alpha: float = 1.0, lanes=None):
     """qsgd_decode of the packed words (summed over `world` ranks) times alpha into
     the gradient tensors, clipped by the norm of all of them; -> that norm
-    before clipping.  The unclipped gradients are never stored."""
+    before clipping.  The unclipped gradients are never stored.  lanes: the
+    words' layout, number of ranks included, where it is not that of
+    qsgd_layout(n, bits, world)."""
     max_norm, code = _limit(max_norm), _norm_code(norm_type)
     dev = _on_gpu(words)
     g = _table(grads, written=True)
