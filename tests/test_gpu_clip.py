@@ -985,3 +985,136 @@ def test_decode_of_large_lists(name, kind, bits, world, p):
     close_norm(total, want, roundings=5)
     close_on_device(torch.cat(outs), x.mul_(coef64(want, 0.37 * want)), extra=8)
     assert bool((buf[between] == 7).all())
+
+
+# ---------------------------------------------------------------------------
+# calls that the documentation allows
+# ---------------------------------------------------------------------------
+def test_the_trainer_call_captured_and_replayed():
+    """clip_grad_norm_ in a graph: replays above and under the limit, eager calls between them."""
+    grads = carve(RAGGED, types_of("mixed", len(RAGGED)), seed=211)
+    params = [torch.nn.Parameter(torch.zeros_like(v)) for v in views(grads)]
+    for w, v in zip(params, views(grads)):
+        w.grad = v
+    clean = [v.clone() for v in views(grads)]
+    limit = 0.5 * norm64(f64(clean), 2)
+    gcodec.clip_grad_norm_(params, limit)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        n = gcodec.clip_grad_norm_(params, limit)
+    for factor in (1.0, 0.25, 4.0, 0.5, 1.0):
+        for v, c in zip(views(grads), clean):
+            v.copy_(c * factor)
+        xs = f64(views(grads))
+        want = norm64(xs, 2)
+        graph.replay()
+        close_norm(gcodec.grad_norm(clean), norm64(f64(clean), 2))
+        torch.cuda.synchronize()
+        close_norm(n, want)
+        close_values(views(grads), [x * coef64(want, limit) for x in xs])
+        guards_hold(grads)
+
+
+def test_two_threads_at_once():
+    """One table and lists of each thread's own, on streams of their own."""
+    import threading
+
+    shared = views(carve([1_000_003, 12, 50_000], [F32, BF16, F16], seed=221))
+    table, want = gcodec.Grads(shared), norm64(f64(shared), 2)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                own = views(carve([70_001, 5, 9000 + seed], [F32, F16, BF16], seed=seed))
+                xs = f64(own)
+                n = norm64(xs, 2)
+                for _ in range(20):
+                    a = gcodec.grad_norm(table)
+                    outs = [torch.empty_like(t) for t in own]
+                    b = gcodec.clip_grads(own, outs, 0.5 * n)
+                    with pytest.raises(gcodec.GCodecError, match=("share memory", "sizes", "tensors into")[seed - 1]):
+                        gcodec.clip_grads(own, (own[:1] * 3, own[::-1], own[:2])[seed - 1], 1.0)  # each its own message
+                    torch.cuda.current_stream().synchronize()
+                    close_norm(a, want)
+                    close_norm(b, n)
+                    close_values(outs, [x * coef64(n, 0.5 * n) for x in xs])
+        except BaseException as e:  # noqa: BLE001 - handed to the test's thread
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if wrong:
+        raise wrong[0]
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+def test_a_tensor_read_twice(p):
+    """A list that is only read may hold a tensor twice, or parts that overlap: each counts."""
+    y = views(carve([9000], [F32], seed=231))[0]
+    ts = [y, y, y[5:7000], y[:0]]
+    xs = f64(ts)
+    n = norm64(xs, p)
+    total, each = gcodec.grad_norm(ts, p, per_tensor=True)
+    close_norm(total, n)
+    for e, x in zip(each.tolist(), xs):
+        close_norm(e, norm64([x], p))
+    flat, peak, total = gcodec.flatten_clip(gcodec.Grads(ts), 0.5 * n, p)
+    close_norm(total, n)
+    close_values([flat], [np.concatenate(xs) * coef64(n, 0.5 * n)])
+    outs = [torch.empty_like(t) for t in ts]
+    gcodec.clip_grads(ts, outs, 0.5 * n, p)
+    close_values(outs, [x * coef64(n, 0.5 * n) for x in xs])
+
+
+@pytest.mark.parametrize("count", [1, 3, 1100])
+def test_decode_of_no_elements(count):
+    outs = [torch.empty(0, device=DEV) for _ in range(count)]
+    words = torch.empty(0, dtype=torch.int32, device=DEV)
+    for scale in (0.02, 0.0, INF, math.nan):
+        norm = torch.tensor([scale], device=DEV)
+        for p in (1, 2, INF):
+            assert float(gcodec.qsgd_decode_clip(words, norm, 4, outs, 1.0, p)) == 0.0
+
+
+@pytest.mark.parametrize("p", [1, 2, INF])
+@pytest.mark.parametrize("bits,world", [(24, 128), (24, 8), (17, 16_000), (1, 2_000_000_000)])
+def test_decode_of_the_widest_lanes(bits, world, p):
+    """Lanes of up to 32 bits, whose sums pass 31: the values are qsgd_decode's, bit for bit."""
+    sizes = [5000, 0, 33, 4001]
+    n, s = sum(sizes), (1 << bits) - 1
+    lanes = codec.qsgd_layout(n, bits, world)
+    assert lanes.per_word == 1 and lanes.bits >= 28
+    rng = np.random.default_rng(241)
+    q = rng.integers(-world * s, world * s + 1, n)
+    q[:3] = world * s, -world * s, 0
+    words = torch.zeros(lanes.plane_words, dtype=torch.int64, device=DEV)
+    words[:n] = torch.from_numpy(q + world * s).to(DEV)
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+    norm = torch.tensor([0.02], device=DEV)
+    dense = codec.qsgd_decode(words, n, norm, bits, world, alpha=1.0 / world)
+    outs = views(carve(sizes, [F32] * len(sizes), seed=242))
+    total = gcodec.qsgd_decode_clip(words, norm, bits, outs, INF, p, world=world, alpha=1.0 / world)
+    assert torch.equal(torch.cat(outs).view(torch.int32), dense.view(torch.int32))
+    want = norm64(f64([dense]), p)
+    close_norm(total, want)
+    # the integers' own: RN(norm / s), RN of the integer to float32, two products, alpha: five roundings, and the norm's
+    close_norm(total, norm64([q * (float(norm) / s / world)], p), roundings=6)
+    gcodec.qsgd_decode_clip(words, norm, bits, outs, 0.5 * want, p, world=world, alpha=1.0 / world)
+    close_values([torch.cat(outs)], [dense.cpu().double().numpy() * coef64(want, 0.5 * want)])
+
+
+def test_decode_takes_the_scale_in_any_form():
+    words, q, norm = packed(5000, 4, 1, seed=251, norm=0.25)
+    want, got = ([torch.empty(5000, device=DEV)] for _ in range(2))
+    gcodec.qsgd_decode_clip(words, norm, 4, want, 1.0)
+    for form in (0.25, norm.double(), norm.cpu(), norm.reshape(()), torch.tensor([0.25, 9.0], device=DEV)[:1],
+                 torch.tensor([[0.25, 9.0]], device=DEV, dtype=torch.float64)):
+        got[0].fill_(9.0)
+        gcodec.qsgd_decode_clip(words, form, 4, got, 1.0)
+        assert torch.equal(want[0], got[0])
