@@ -1110,8 +1110,9 @@ static int check_sides(const Side (&side)[N], const gc_grads *src, const gc_grad
             continue;
         for (size_t j = i + 1; j < N; ++j) {
             const uint64_t at = reinterpret_cast<uint64_t>(side[j].at);
-            GC_REQUIRE(!(side[i].written || side[j].written) || !at || at >= x.hi || at + side[j].bytes <= x.lo,
-                       "%s: %s and %s share memory", what, side[i].name, side[j].name);
+            const bool apart = !at || side[j].bytes == 0 || at >= x.hi || at + side[j].bytes <= x.lo;
+            GC_REQUIRE(apart || !(side[i].written || side[j].written), "%s: %s and %s share memory", what,
+                       side[i].name, side[j].name);
         }
         uint64_t at = 0;
         GC_REQUIRE(!(src && side[i].written && meets(src, x, &at)), "%s: %s shares memory with input tensor %llu", what,

@@ -1118,3 +1118,16 @@ def test_decode_takes_the_scale_in_any_form():
         got[0].fill_(9.0)
         gcodec.qsgd_decode_clip(words, form, 4, got, 1.0)
         assert torch.equal(want[0], got[0])
+
+
+def test_a_workspace_of_no_bytes_shares_no_memory():
+    """A short list's workspace may point anywhere, also into the bucket."""
+    from gcodec import _lib
+
+    lib = _lib.load()
+    ts = views(carve([1000, 3], [F32, BF16], seed=261))
+    g, want = gcodec.Grads(ts), gcodec.flatten_clip(ts, 0.5)
+    flat, peak, norm = torch.empty(g.n, device=DEV), torch.zeros(1, device=DEV), torch.zeros((), device=DEV)
+    assert lib.gc_grad_flatten_clip(g._ref, flat.data_ptr(), 2, 0.5, peak.data_ptr(), norm.data_ptr(),
+                                    flat.data_ptr() + 64, torch.cuda.current_stream().cuda_stream) == 0, _lib.last_error()
+    assert torch.equal(flat, want[0]) and torch.equal(peak, want[1]) and torch.equal(norm, want[2])
